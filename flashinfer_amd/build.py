@@ -1,9 +1,11 @@
 """Builds libmi_moe.so (all HIP kernels + the C ABI, for the default
 definition: H=7168, I=2048, 32 of 256 experts, 8 groups, top-4 groups,
 top-8), one libmi_moe_<tag>.so per further definition in
-shapes.DEFINITIONS, and libmi_peaks.so (achievable-peak probes used by
-bench.py), for gfx950 with hipcc; and _mi_moe_host, the native host path of
-kernel.run (host C++ against torch's headers, built with g++).
+shapes.DEFINITIONS, libmi_experts.so (the operators around the experts, for
+any sizes), and libmi_peaks.so (achievable-peak probes used by bench.py), for
+gfx950 with hipcc; and two extensions of host C++ against torch's headers,
+built with g++: _mi_moe_host, the native host path of kernel.run, and
+_mi_experts, the torch side of the expert operators.
 
 Usage: python -m flashinfer_amd.build [--jobs N] [--save-temps]
 The shared libraries land next to this file so they travel with the tree.
@@ -26,6 +28,10 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmi_moe.so")
 SOURCES = ["route.hip", "sort.hip", "gemm1.hip", "gemm2.hip", "gemm1_tile.hip", "gemm2_tile.hip",
            "gemm1_wide.hip", "gemm2_wide.hip", "gemm2_combine.hip", "combine.hip", "quant.hip", "capi.hip"]
+# operators whose sizes are arguments: one library for all definitions
+EXPERTS_LIB = os.path.join(HERE, "libmi_experts.so")
+EXPERTS_SOURCES = ["experts_sort.hip", "experts_move.hip", "int8_quant.hip", "int8_gemm.hip",
+                   "experts_capi.hip"]
 PEAKS_LIB = os.path.join(HERE, "libmi_peaks.so")
 PEAKS_SOURCES = ["peaks.hip"]
 # Per-source flags: MFMA results in VGPRs rather than AGPRs.
@@ -89,30 +95,42 @@ def _link(objs, out):
 
 HOST_SRC = os.path.join(CSRC, "host_bind.cpp")
 HOST_LIB = os.path.join(HERE, "_mi_moe_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+EXPERTS_SRC = os.path.join(CSRC, "experts_bind.cpp")
+EXPERTS_EXT = os.path.join(HERE, "_mi_experts" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def build_host() -> str:
-    """The torch extension _mi_moe_host: host code only, so g++ builds it
-    (against torch's headers and its bundled pybind11) without hipcc."""
+def _build_extension(src: str, out: str, links) -> str:
+    """A torch extension of host code only, so g++ builds it (against torch's
+    headers and its bundled pybind11) without hipcc."""
     import torch
     tdir = os.path.dirname(torch.__file__)
     tlib = os.path.join(tdir, "lib")
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    tmp = HOST_LIB + ".tmp"
+    tmp = out + ".tmp"
     cmd = [shutil.which("g++") or "g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
            "-I", os.path.join(tdir, "include"),
            "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(rocm, "include"),
-           HOST_SRC, "-o", tmp, "-L", tlib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+           src, "-o", tmp, *links, "-L", tlib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
            "-ltorch_python", "-L", os.path.join(rocm, "lib"), "-lamdhip64",
-           f"-Wl,-rpath,{tlib}"]
+           f"-Wl,-rpath,$ORIGIN:{tlib}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on host_bind.cpp:\n{r.stderr}")
-    os.replace(tmp, HOST_LIB)
-    return HOST_LIB
+        raise RuntimeError(f"g++ failed on {os.path.basename(src)}:\n{r.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
+def build_host() -> str:
+    """_mi_moe_host: the native host path of kernel.run."""
+    return _build_extension(HOST_SRC, HOST_LIB, [])
+
+
+def build_experts_ext() -> str:
+    """_mi_experts: the torch side of the expert operators, linked to libmi_experts.so."""
+    return _build_extension(EXPERTS_SRC, EXPERTS_EXT, ["-L", HERE, "-l:" + os.path.basename(EXPERTS_LIB)])
 
 
 def build(jobs: int = 8, extra=()) -> str:
@@ -120,14 +138,19 @@ def build(jobs: int = 8, extra=()) -> str:
     if bad:
         raise ValueError(f"unsupported definitions (see shapes.py): {bad}")
     os.makedirs(BUILD, exist_ok=True)
-    jobs_list = [(s, d) for d in DEFINITIONS for s in SOURCES] + [(s, None) for s in PEAKS_SOURCES]
+    jobs_list = ([(s, d) for d in DEFINITIONS for s in SOURCES] + [(s, None) for s in EXPERTS_SOURCES]
+                 + [(s, None) for s in PEAKS_SOURCES])
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         objs = list(ex.map(lambda j: _compile(j[0], list(extra), j[1]), jobs_list))
     n = len(SOURCES)
     for k, d in enumerate(DEFINITIONS):
         _link(objs[k * n:(k + 1) * n], os.path.join(HERE, lib_name_of(d)))
-    _link(objs[len(DEFINITIONS) * n:], PEAKS_LIB)
-    build_host()
+    rest = objs[len(DEFINITIONS) * n:]
+    _link(rest[:len(EXPERTS_SOURCES)], EXPERTS_LIB)
+    _link(rest[len(EXPERTS_SOURCES):], PEAKS_LIB)
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        for done in [ex.submit(build_host), ex.submit(build_experts_ext)]:
+            done.result()
     return LIB
 
 

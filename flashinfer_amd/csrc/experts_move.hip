@@ -1,0 +1,256 @@
+// Token rows to expert order and back (mi_experts_permute, _unpermute,
+// _unpermute_backward).
+//
+// All three go by token: a token's row and its k places are read once, and the
+// k rows that belong to it are written (or gathered) from there, so the
+// smaller side of the traffic crosses HBM once and no row index has to be
+// inverted. The sums over a token's slots and over a row's columns run in
+// fp32 in a fixed order; no atomics. All are bound by HBM.
+//
+// tx = 2^tx_log lanes share a token (as many as its row has vectors, at most
+// a workgroup), so short rows still fill the waves.
+#include "experts_common.hpp"
+
+namespace miexp {
+
+constexpr int THREADS = 256;
+constexpr int KG = 8;  // slots of a token handled together
+
+inline int lanes_log(int64_t vectors) {
+    int l = 0;
+    while (l < 8 && (1ll << l) < vectors) ++l;
+    return l;
+}
+
+inline unsigned blocks_for(int64_t T, int tx_log) {
+    const int64_t b = (T + (THREADS >> tx_log) - 1) / (THREADS >> tx_log);
+    return (unsigned)(b < MAX_BLOCKS ? b : MAX_BLOCKS);
+}
+
+// V: the unit that moves, as wide as row length, strides and addresses allow.
+template <class V>
+__global__ __launch_bounds__(THREADS) void permute_kernel(const char* __restrict__ x, int64_t x_stride,
+                                                          int64_t T, int k, int64_t vectors,
+                                                          const int32_t* __restrict__ row_of_slot,
+                                                          const int32_t* __restrict__ num_rows,
+                                                          char* __restrict__ rows, int64_t rows_stride,
+                                                          int zero_rest, int tx_log) {
+    const int tx = 1 << tx_log;
+    const int64_t R = T * k;
+    const int64_t local = min((int64_t)*num_rows, R);
+    const int64_t v = (int64_t)blockIdx.y * tx + (threadIdx.x & (tx - 1));
+    if (v >= vectors) return;
+    for (int64_t t = (int64_t)blockIdx.x * (THREADS >> tx_log) + (threadIdx.x >> tx_log); t < T;
+         t += (int64_t)gridDim.x * (THREADS >> tx_log)) {
+        const V val = reinterpret_cast<const V*>(x + t * x_stride)[v];
+        for (int j = 0; j < k; ++j) {
+            const int64_t row = row_of_slot[t * k + j];
+            if (row >= 0 && row < local)
+                reinterpret_cast<V*>(rows + row * rows_stride)[v] = val;
+            else if (zero_rest && row >= 0 && row < R)
+                reinterpret_cast<V*>(rows + row * rows_stride)[v] = V{};
+        }
+    }
+}
+
+hipError_t launch_permute(const void* x, int64_t x_stride, int64_t T, int k, int64_t row_bytes,
+                          const int32_t* row_of_slot, const int32_t* num_rows, void* rows,
+                          int64_t rows_stride, bool zero_rest, hipStream_t s) {
+    const uint64_t bits = (uint64_t)x | (uint64_t)rows | (uint64_t)x_stride | (uint64_t)rows_stride |
+                          (uint64_t)row_bytes;
+    auto go = [&](auto unit) {
+        typedef decltype(unit) V;
+        const int64_t vectors = row_bytes / (int64_t)sizeof(V);
+        const int tx_log = lanes_log(vectors);
+        const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
+        hipLaunchKernelGGL((permute_kernel<V>), grid, dim3(THREADS), 0, s, (const char*)x, x_stride, T, k,
+                           vectors, row_of_slot, num_rows, (char*)rows, rows_stride, (int)zero_rest, tx_log);
+        return hipGetLastError();
+    };
+    if (bits % 16 == 0) return go(v4i{});
+    if (bits % 8 == 0) return go((uint64_t)0);
+    if (bits % 4 == 0) return go((uint32_t)0);
+    if (bits % 2 == 0) return go((uint16_t)0);
+    return go((uint8_t)0);
+}
+
+template <class T, int N, bool WEIGHTED>
+__global__ __launch_bounds__(THREADS) void unpermute_kernel(const T* __restrict__ rows, int64_t rows_stride,
+                                                            int64_t tokens, int k, int64_t H,
+                                                            const int32_t* __restrict__ row_of_slot,
+                                                            const int32_t* __restrict__ num_rows,
+                                                            const float* __restrict__ weights,
+                                                            T* __restrict__ out, int64_t out_stride,
+                                                            int tx_log) {
+    const int tx = 1 << tx_log;
+    const int64_t local = min((int64_t)*num_rows, tokens * k);
+    const int64_t c = ((int64_t)blockIdx.y * tx + (threadIdx.x & (tx - 1))) * N;
+    if (c >= H) return;
+    for (int64_t t = (int64_t)blockIdx.x * (THREADS >> tx_log) + (threadIdx.x >> tx_log); t < tokens;
+         t += (int64_t)gridDim.x * (THREADS >> tx_log)) {
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        for (int j0 = 0; j0 < k; j0 += KG) {
+            float v[KG][N], w[KG];
+            bool on[KG];
+#pragma unroll
+            for (int j = 0; j < KG; ++j) {
+                const bool in = j0 + j < k;
+                const int64_t row = in ? row_of_slot[t * k + j0 + j] : -1;
+                on[j] = row >= 0 && row < local;
+                w[j] = 1.f;
+                if (on[j]) {
+                    load<T, N>(rows + row * rows_stride + c, v[j]);
+                    if (WEIGHTED) w[j] = weights[t * k + j0 + j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < KG; ++j)
+                if (on[j]) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        acc[i] = WEIGHTED ? fmaf(w[j], v[j][i], acc[i]) : acc[i] + v[j][i];
+                }
+        }
+        store<T, N>(out + t * out_stride + c, acc);
+    }
+}
+
+// Gradients of a token's rows and weights: its tx lanes walk the columns, each
+// lane keeps one partial product sum per slot, and the sums meet at the end.
+template <class T, int N>
+__global__ __launch_bounds__(THREADS) void unpermute_backward_kernel(
+    const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ rows, int64_t rows_stride,
+    int64_t tokens, int k, int64_t H, const int32_t* __restrict__ row_of_slot,
+    const int32_t* __restrict__ num_rows, const float* __restrict__ weights, T* __restrict__ grad_rows,
+    int64_t grad_rows_stride, int zero_rest, float* __restrict__ grad_weights, int tx_log) {
+    __shared__ float part[THREADS / 64][KG];
+    const int tx = 1 << tx_log, lane = threadIdx.x & (tx - 1);
+    const int64_t R = tokens * k;
+    const int64_t local = min((int64_t)*num_rows, R);
+    const int64_t per = THREADS >> tx_log;
+    // the same number of rounds for all threads: they meet at the barriers
+    for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tokens; t0 += (int64_t)gridDim.x * per) {
+        const int64_t t = t0 + (threadIdx.x >> tx_log);
+        const bool live = t < tokens;
+        for (int j0 = 0; j0 < k; j0 += KG) {
+            int64_t row[KG];
+            float w[KG], dot[KG];
+#pragma unroll
+            for (int j = 0; j < KG; ++j) {
+                row[j] = live && j0 + j < k ? row_of_slot[t * k + j0 + j] : -1;
+                if (row[j] >= R) row[j] = -1;
+                w[j] = row[j] >= 0 && weights ? weights[t * k + j0 + j] : 1.f;
+                dot[j] = 0.f;
+            }
+            if (live) {
+                for (int64_t c = (int64_t)lane * N; c < H; c += (int64_t)tx * N) {
+                    float g[N];
+                    load<T, N>(grad + t * grad_stride + c, g);
+#pragma unroll
+                    for (int j = 0; j < KG; ++j) {
+                        if (row[j] < 0) continue;
+                        if (row[j] < local) {
+                            if (grad_weights) {
+                                float v[N];
+                                load<T, N>(rows + row[j] * rows_stride + c, v);
+#pragma unroll
+                                for (int i = 0; i < N; ++i) dot[j] = fmaf(g[i], v[i], dot[j]);
+                            }
+                            if (grad_rows) {
+                                float d[N];
+#pragma unroll
+                                for (int i = 0; i < N; ++i) d[i] = w[j] * g[i];
+                                store<T, N>(grad_rows + row[j] * grad_rows_stride + c, d);
+                            }
+                        } else if (grad_rows && zero_rest) {
+                            float d[N];
+#pragma unroll
+                            for (int i = 0; i < N; ++i) d[i] = 0.f;
+                            store<T, N>(grad_rows + row[j] * grad_rows_stride + c, d);
+                        }
+                    }
+                }
+            }
+            if (!grad_weights) continue;
+            for (int d = min(tx, 64) >> 1; d >= 1; d >>= 1)
+#pragma unroll
+                for (int j = 0; j < KG; ++j) dot[j] += __shfl_xor(dot[j], d);
+            if (tx > 64) {
+                if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                    for (int j = 0; j < KG; ++j) part[threadIdx.x >> 6][j] = dot[j];
+                __syncthreads();
+                const int w0 = (threadIdx.x >> tx_log) * (tx >> 6);
+#pragma unroll
+                for (int j = 0; j < KG; ++j) {
+                    dot[j] = 0.f;
+                    for (int w1 = 0; w1 < tx >> 6; ++w1) dot[j] += part[w0 + w1][j];
+                }
+                __syncthreads();
+            }
+            if (live && lane == 0)
+#pragma unroll
+                for (int j = 0; j < KG; ++j)
+                    if (j0 + j < k) grad_weights[t * k + j0 + j] = dot[j];
+        }
+    }
+}
+
+// Calls go(T{}, IntC<N>{}) with the widest vector (16 bytes, else 1 element)
+// that the row length, strides (in elements) and addresses allow.
+template <int N> struct IntC { static constexpr int value = N; };
+
+template <class F>
+hipError_t by_type(int dtype, uint64_t elems, uint64_t addresses, F go) {
+    const int size = dtype == MI_EXPERTS_F32 ? 4 : 2;
+    const bool wide = (elems * size) % 16 == 0 && addresses % 16 == 0;
+    if (dtype == MI_EXPERTS_F32) return wide ? go(float{}, IntC<4>{}) : go(float{}, IntC<1>{});
+    if (dtype == MI_EXPERTS_F16) return wide ? go(_Float16{}, IntC<8>{}) : go(_Float16{}, IntC<1>{});
+    return wide ? go(__bf16{}, IntC<8>{}) : go(__bf16{}, IntC<1>{});
+}
+
+hipError_t launch_unpermute(int dtype, const void* rows, int64_t rows_stride, int64_t T, int k, int64_t H,
+                            const int32_t* row_of_slot, const int32_t* num_rows, const float* weights,
+                            void* out, int64_t out_stride, hipStream_t s) {
+    return by_type(dtype, (uint64_t)rows_stride | (uint64_t)out_stride | (uint64_t)H,
+                   (uint64_t)rows | (uint64_t)out, [&](auto elem, auto width) {
+        typedef decltype(elem) E;
+        constexpr int N = decltype(width)::value;
+        const int64_t vectors = (H + N - 1) / N;
+        const int tx_log = lanes_log(vectors);
+        const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
+        if (weights)
+            hipLaunchKernelGGL((unpermute_kernel<E, N, true>), grid, dim3(THREADS), 0, s, (const E*)rows,
+                               rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)out, out_stride,
+                               tx_log);
+        else
+            hipLaunchKernelGGL((unpermute_kernel<E, N, false>), grid, dim3(THREADS), 0, s, (const E*)rows,
+                               rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)out, out_stride,
+                               tx_log);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_unpermute_backward(int dtype, const void* grad, int64_t grad_stride, const void* rows,
+                                     int64_t rows_stride, int64_t T, int k, int64_t H,
+                                     const int32_t* row_of_slot, const int32_t* num_rows,
+                                     const float* weights, void* grad_rows, int64_t grad_rows_stride,
+                                     bool zero_rest, float* grad_weights, hipStream_t s) {
+    const uint64_t elems = (uint64_t)grad_stride | (uint64_t)H | (grad_weights ? (uint64_t)rows_stride : 0) |
+                           (grad_rows ? (uint64_t)grad_rows_stride : 0);
+    const uint64_t addr = (uint64_t)grad | (grad_weights ? (uint64_t)rows : 0) | (uint64_t)grad_rows;
+    return by_type(dtype, elems, addr, [&](auto elem, auto width) {
+        typedef decltype(elem) E;
+        constexpr int N = decltype(width)::value;
+        const int tx_log = lanes_log((H + N - 1) / N);
+        hipLaunchKernelGGL((unpermute_backward_kernel<E, N>), dim3(blocks_for(T, tx_log)), dim3(THREADS), 0,
+                           s, (const E*)grad, grad_stride, (const E*)rows, rows_stride, T, k, H, row_of_slot,
+                           num_rows, weights, (E*)grad_rows, grad_rows_stride, (int)zero_rest, grad_weights,
+                           tx_log);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace miexp

@@ -1,0 +1,227 @@
+// Slots sorted by local expert: a stable counting sort of T * k ids into E + 1
+// buckets, the last of which takes the ids of other shards.
+//
+//   row(slot) = #{slots in lower buckets} + #{earlier slots in its bucket}
+//
+// The second term is found a wave at a time: lanes with equal buckets find
+// each other by one ballot per bit of the bucket, a lane's place among them is
+// the count of equal lanes below it, and the lowest of them advances the
+// bucket's counter in LDS. Counters belong to one wave each and waves take
+// contiguous slots, so the order is that of the slots and no result hangs on
+// the order of atomics.
+//
+// Up to SMALL slots one workgroup does it all (the latency of three passes
+// over LDS). Beyond, one launch counts the buckets of at most 256 chunks, and
+// a second one places them: each workgroup sums the counts of the chunks
+// before its own, which are in L2.
+#include "experts_common.hpp"
+
+namespace miexp {
+
+constexpr int64_t SMALL = 8192;
+constexpr int64_t MAX_CHUNKS = 256;
+constexpr int CHUNK_MIN = 2048;
+
+__host__ __device__ inline int64_t chunk_len(int64_t slots) {
+    const int64_t per = (slots + MAX_CHUNKS - 1) / MAX_CHUNKS;
+    return per <= CHUNK_MIN ? CHUNK_MIN : (per + 1023) / 1024 * 1024;
+}
+
+int64_t sort_chunks(int64_t slots) {
+    if (slots <= SMALL) return 0;
+    const int64_t len = chunk_len(slots);
+    return (slots + len - 1) / len;
+}
+
+__device__ __forceinline__ int bucket_of(int id, long long offset, int E) {
+    const long long l = (long long)id - offset;
+    return l >= 0 && l < E ? (int)l : E;
+}
+
+// Lanes of the wave whose bucket is this lane's, among those with `live`.
+__device__ __forceinline__ unsigned long long same_bucket(int b, int bits, bool live) {
+    unsigned long long m = __ballot(live);
+    for (int i = 0; i < bits; ++i) {
+        const unsigned long long on = __ballot((b >> i) & 1);
+        m &= (b >> i) & 1 ? on : ~on;
+    }
+    return m;
+}
+
+// Exclusive scan over the workgroup's threads of one value each; *total gets
+// the sum. `tmp` holds a value per wave.
+__device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int inc = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(inc, d);
+        if (lane >= d) inc += u;
+    }
+    if (lane == 63) tmp[wave] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < waves; ++w) {
+        const int u = tmp[w];
+        if (w < wave) before += u;
+        all += u;
+    }
+    *total = all;
+    __syncthreads();
+    return before + inc - v;
+}
+
+// Places slots [first, last) whose buckets start at base[b] (b < E + 1 <= 1025,
+// one or two per thread). counts: LDS [waves][E + 1].
+__device__ void place(const int32_t* ids, int64_t first, int64_t last, int k, int E, long long offset,
+                      int bits, int* counts, const int* base, int32_t* token_of_row,
+                      int32_t* row_of_slot) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int64_t per = ((last - first + waves - 1) / waves + 63) / 64 * 64;
+    const int64_t a = first + wave * per, z = min(a + per, last);
+    int* mine = counts + wave * (E + 1);
+    for (int i = threadIdx.x; i < waves * (E + 1); i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    for (int64_t s = a; s < z; s += 64) {
+        const bool live = s + lane < z;
+        const int b = live ? bucket_of(ids[s + lane], offset, E) : 0;
+        const unsigned long long m = same_bucket(b, bits, live);
+        if (live && lane == __ffsll(m) - 1) atomicAdd(&mine[b], __popcll(m));
+    }
+    __syncthreads();
+    // counts -> first row of each wave's part of a bucket
+    for (int b = threadIdx.x; b <= E; b += blockDim.x) {
+        int at = base[b];
+        for (int w = 0; w < waves; ++w) {
+            const int c = counts[w * (E + 1) + b];
+            counts[w * (E + 1) + b] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (int64_t s = a; s < z; s += 64) {
+        const bool live = s + lane < z;
+        const int b = live ? bucket_of(ids[s + lane], offset, E) : 0;
+        const unsigned long long m = same_bucket(b, bits, live);
+        const int lead = m ? __ffsll(m) - 1 : 0;
+        int at = 0;
+        if (live && lane == lead) at = atomicAdd(&mine[b], __popcll(m));
+        at = __shfl(at, lead);
+        if (live) {
+            const int row = at + __popcll(m & ((1ull << lane) - 1));
+            row_of_slot[s + lane] = row;
+            token_of_row[row] = (int32_t)((s + lane) / k);
+        }
+    }
+}
+
+// One workgroup. LDS: base [E + 1], counts [waves][E + 1], 16 wave sums.
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int32_t* __restrict__ ids, int n, int k,
+                                                          int E, long long offset, int bits,
+                                                          int32_t* __restrict__ offsets,
+                                                          int32_t* __restrict__ token_of_row,
+                                                          int32_t* __restrict__ row_of_slot) {
+    extern __shared__ int smem[];
+    int* base = smem;
+    int* counts = base + (E + 1);
+    int* tmp = counts + (blockDim.x >> 6) * (E + 1);
+    for (int i = threadIdx.x; i <= E; i += blockDim.x) base[i] = 0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < n; s += blockDim.x) atomicAdd(&base[bucket_of(ids[s], offset, E)], 1);
+    __syncthreads();
+    int before = 0;
+    for (int b0 = 0; b0 < E; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        int total;
+        const int at = before + block_scan(b < E ? base[b] : 0, tmp, &total);
+        if (b < E) {
+            offsets[b] = at;
+            base[b] = at;
+        }
+        before += total;
+    }
+    if (threadIdx.x == 0) {
+        offsets[E] = before;
+        base[E] = before;
+    }
+    __syncthreads();
+    place(ids, 0, n, k, E, offset, bits, counts, base, token_of_row, row_of_slot);
+}
+
+__global__ __launch_bounds__(512) void sort_count_kernel(const int32_t* __restrict__ ids, int64_t n,
+                                                         int64_t len, int E, long long offset,
+                                                         int32_t* __restrict__ chunk_counts) {
+    extern __shared__ int smem[];
+    for (int i = threadIdx.x; i <= E; i += blockDim.x) smem[i] = 0;
+    __syncthreads();
+    const int64_t a = blockIdx.x * len, z = min(a + len, n);
+    for (int64_t s = a + threadIdx.x; s < z; s += blockDim.x)
+        atomicAdd(&smem[bucket_of(ids[s], offset, E)], 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i <= E; i += blockDim.x) chunk_counts[(int64_t)blockIdx.x * (E + 1) + i] = smem[i];
+}
+
+__global__ __launch_bounds__(512) void sort_place_kernel(const int32_t* __restrict__ ids, int64_t n,
+                                                         int64_t len, int k, int E, long long offset,
+                                                         int bits, const int32_t* __restrict__ chunk_counts,
+                                                         int32_t* __restrict__ offsets,
+                                                         int32_t* __restrict__ token_of_row,
+                                                         int32_t* __restrict__ row_of_slot) {
+    extern __shared__ int smem[];
+    int* base = smem;
+    int* counts = base + (E + 1);
+    int* tmp = counts + (blockDim.x >> 6) * (E + 1);
+    int before = 0;  // rows of the buckets below this step's
+    for (int b0 = 0; b0 <= E; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        int prior = 0, all = 0;
+        if (b <= E) {
+#pragma unroll 8
+            for (int c = 0; c < (int)gridDim.x; ++c) {
+                const int v = chunk_counts[(int64_t)c * (E + 1) + b];
+                if (c < (int)blockIdx.x) prior += v;
+                all += v;
+            }
+        }
+        int total;
+        const int at = before + block_scan(all, tmp, &total);
+        if (b <= E) {
+            base[b] = at + prior;
+            if (blockIdx.x == 0) offsets[b] = at;
+        }
+        before += total;
+    }
+    __syncthreads();
+    const int64_t a = blockIdx.x * len;
+    place(ids, a, min(a + len, n), k, E, offset, bits, counts, base, token_of_row, row_of_slot);
+}
+
+hipError_t launch_sort(const int32_t* ids, int64_t T, int k, int E, int64_t offset, int32_t* offsets,
+                       int32_t* token_of_row, int32_t* row_of_slot, int32_t* counts, hipStream_t s) {
+    const int64_t n = T * k;
+    int bits = 0;
+    while ((E >> bits) != 0) ++bits;
+    const int64_t chunks = sort_chunks(n);
+    if (chunks == 0) {
+        // a wave per 64 slots, enough threads to scan the buckets, LDS within 64 KB
+        int waves = (int)((n + 63) / 64), scan = (E + 63) / 64;
+        if (scan > 4) scan = 4;
+        if (waves < scan) waves = scan;
+        const int most = (int)((65536 - 64) / sizeof(int)) / (E + 1) - 1;
+        if (waves > most) waves = most;
+        if (waves > 16) waves = 16;
+        const size_t lds = ((size_t)(waves + 1) * (E + 1) + 16) * sizeof(int);
+        hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(64 * waves), lds, s, ids, (int)n, k, E,
+                           (long long)offset, bits, offsets, token_of_row, row_of_slot);
+        return hipGetLastError();
+    }
+    const int64_t len = chunk_len(n);
+    hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)chunks), dim3(512), (E + 1) * sizeof(int), s, ids,
+                       n, len, E, (long long)offset, counts);
+    const size_t lds = ((size_t)9 * (E + 1) + 16) * sizeof(int);
+    hipLaunchKernelGGL(sort_place_kernel, dim3((unsigned)chunks), dim3(512), lds, s, ids, n, len, k, E,
+                       (long long)offset, bits, counts, offsets, token_of_row, row_of_slot);
+    return hipGetLastError();
+}
+
+}  // namespace miexp

@@ -1,0 +1,130 @@
+// Rows of floats to int8 with a scale each (mi_experts_quantize_int8), and the
+// same after SwiGLU.
+//
+//   scale[m] = max(amax, 1e-10) / 127,  q = rint(x / scale)
+//
+// The largest magnitude is found over the bits of |x|, whose order as integers
+// is that of the floats with infinities and NaN on top: a row that holds one
+// gets a scale that is not finite, and zeros, so that its products are NaN
+// instead of numbers made without it.
+//
+// A wave (rows up to 1024 elements) or a workgroup takes a row. Its first
+// CACHED vectors per lane stay in registers between the two passes; longer
+// rows are read (and, with SwiGLU, computed) again from L2. Bound by HBM.
+#include "experts_common.hpp"
+
+namespace miexp {
+
+constexpr float INT8_MAX_F = 127.f;
+constexpr float QUANT_FLOOR = 1e-10f;  // scale of an all-zero row: that of quantize_activations
+
+template <class T, int N, bool SWIGLU>
+__device__ __forceinline__ void quant_input(const T* row, int64_t K, int64_t c, float (&v)[N]) {
+    load<T, N>(row + c, v);
+    if constexpr (SWIGLU) {
+        float u[N];
+        load<T, N>(row + K + c, u);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= u[i] / (1.f + expf(-u[i]));
+    }
+}
+
+template <class T, int N, bool SWIGLU, int CACHED, int TX>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t x_stride, int64_t M,
+                                                       int64_t K, const int32_t* __restrict__ num_rows,
+                                                       int8_t* __restrict__ q, int64_t q_stride,
+                                                       float* __restrict__ scale) {
+    constexpr int ROWS = 256 / TX;
+    __shared__ uint32_t part[4];
+    const int lane = threadIdx.x & (TX - 1);
+    if (num_rows) M = min(M, (int64_t)*num_rows);
+    for (int64_t m0 = (int64_t)blockIdx.x * ROWS; m0 < M; m0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t m = m0 + threadIdx.x / TX;
+        const bool live = m < M;
+        const T* row = x + (live ? m : 0) * x_stride;
+        float v[CACHED][N];
+        uint32_t top = 0;
+        auto take = [&](const float (&w)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(w[i]) & 0x7fffffffu);
+        };
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < CACHED; ++i) {
+                const int64_t c = ((int64_t)i * TX + lane) * N;
+                if (c < K) quant_input<T, N, SWIGLU>(row, K, c, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < CACHED; ++i)
+                if (((int64_t)i * TX + lane) * N < K) take(v[i]);
+            for (int64_t c = ((int64_t)CACHED * TX + lane) * N; c < K; c += (int64_t)TX * N) {
+                float w[N];
+                quant_input<T, N, SWIGLU>(row, K, c, w);
+                take(w);
+            }
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        if constexpr (TX > 64) {
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+            __syncthreads();
+            top = max(max(part[0], part[1]), max(part[2], part[3]));
+            __syncthreads();
+        }
+        if (!live) continue;
+        const bool finite = top < 0x7f800000u;
+        const float amax = __uint_as_float(top);
+        const float s = finite ? fmaxf(amax, QUANT_FLOOR) / INT8_MAX_F : amax;
+        auto put = [&](int64_t c, const float (&w)[N]) {
+            int8_t b[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) b[i] = finite ? (int8_t)(int)rintf(w[i] / s) : (int8_t)0;
+            if constexpr (N == 8)
+                *reinterpret_cast<uint2*>(q + m * q_stride + c) = *reinterpret_cast<const uint2*>(b);
+            else if constexpr (N == 4)
+                *reinterpret_cast<uint32_t*>(q + m * q_stride + c) = *reinterpret_cast<const uint32_t*>(b);
+            else
+                q[m * q_stride + c] = b[0];
+        };
+#pragma unroll
+        for (int i = 0; i < CACHED; ++i) {
+            const int64_t c = ((int64_t)i * TX + lane) * N;
+            if (c < K) put(c, v[i]);
+        }
+        for (int64_t c = ((int64_t)CACHED * TX + lane) * N; c < K; c += (int64_t)TX * N) {
+            float w[N];
+            quant_input<T, N, SWIGLU>(row, K, c, w);
+            put(c, w);
+        }
+        if (lane == 0) scale[m] = s;
+    }
+}
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+hipError_t launch_quantize(int dtype, const void* x, int64_t x_stride, int64_t M, int64_t K, bool swiglu,
+                           const int32_t* num_rows, int8_t* q, int64_t q_stride, float* scale,
+                           hipStream_t s) {
+    auto go = [&](auto elem, auto wide) {
+        typedef decltype(elem) E;
+        constexpr int N = decltype(wide)::value ? 16 / (int)sizeof(E) : 1;
+        auto launch = [&](auto kernel, int rows) {
+            const int64_t b = (M + rows - 1) / rows;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(b < MAX_BLOCKS ? b : MAX_BLOCKS)), dim3(256), 0, s,
+                               (const E*)x, x_stride, M, K, num_rows, q, q_stride, scale);
+            return hipGetLastError();
+        };
+        if (K <= 1024)
+            return swiglu ? launch(quantize_kernel<E, N, true, 2, 64>, 4) : launch(quantize_kernel<E, N, false, 2, 64>, 4);
+        return swiglu ? launch(quantize_kernel<E, N, true, 4, 256>, 1) : launch(quantize_kernel<E, N, false, 4, 256>, 1);
+    };
+    const uint64_t size = dtype == MI_EXPERTS_F32 ? 4 : 2;
+    const bool wide = (((uint64_t)x_stride | (uint64_t)K) * size) % 16 == 0 && (uint64_t)x % 16 == 0 &&
+                      ((uint64_t)q | (uint64_t)q_stride) % 8 == 0;
+    if (dtype == MI_EXPERTS_F32) return wide ? go(float{}, Yes{}) : go(float{}, No{});
+    if (dtype == MI_EXPERTS_F16) return wide ? go(_Float16{}, Yes{}) : go(_Float16{}, No{});
+    return wide ? go(__bf16{}, Yes{}) : go(__bf16{}, No{});
+}
+
+}  // namespace miexp

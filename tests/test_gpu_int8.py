@@ -1,0 +1,356 @@
+"""The int8 quantisers and products (flashinfer_amd.int8) against 64-bit
+formulas: the plain quantiser bit for bit, products within the roundings of
+their fp32 epilogue and of the result."""
+import pytest
+import torch
+
+import flashinfer_amd as fa
+
+pytestmark = pytest.mark.gpu
+F64 = torch.float64
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _ints(shape, seed, lo=-128):
+    return torch.empty(shape, dtype=torch.int8, device="cuda").random_(lo, 128, generator=_gen(seed))
+
+
+def _scales(shape, seed):
+    return torch.empty(shape, device="cuda").uniform_(0.0005, 0.002, generator=_gen(seed))
+
+
+def _check(got, acc, sa, sb, bias=None):
+    """|got - exact| within: int32 to fp32, two products, the bias's sum, the last rounding."""
+    y = acc * sa.to(F64)[:, None] * sb.to(F64)
+    ref = y if bias is None else y + bias.to(F64)
+    eps = torch.finfo(got.dtype).eps / 2
+    before = 3.001 * U * y.abs() + (U * ref.abs() * 1.001 if bias is not None else 0)
+    bound = before * (1 + eps) + ref.abs() * eps + torch.finfo(got.dtype).smallest_normal * eps * 2
+    bad = (got.to(F64) - ref).abs() > bound
+    assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+def _exact(a, b):
+    return torch.matmul(a.to(F64), b.to(F64).t())  # whole numbers below 2^53: exact
+
+
+SHAPES = [  # M, N, K
+    (1, 1, 1), (1, 16, 64), (1, 4096, 7168), (2, 100, 4096), (3, 17, 33), (5, 64, 128), (16, 4096, 2048),
+    (17, 130, 1024), (31, 48, 272), (33, 1000, 528), (64, 256, 7168), (65, 64, 16), (100, 7168, 2048),
+    (128, 128, 128), (130, 515, 1040), (200, 4096, 512), (256, 256, 256), (257, 300, 130), (300, 264, 784),
+    (511, 513, 96), (600, 1024, 2048), (1024, 2048, 1024), (1111, 999, 400), (2050, 1536, 4096), (4097, 31, 160)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_matmul(shape, dtype):
+    M, N, K = shape
+    a, b, sa, sb = _ints((M, K), 1), _ints((N, K), 2), _scales(M, 3), _scales(N, 4)
+    acc = _exact(a, b)
+    y = fa.int8_matmul(a, sa, b, sb, out_dtype=dtype)
+    assert y.dtype == dtype and y.shape == (M, N)
+    _check(y, acc, sa, sb)
+    bias = torch.randn(N, generator=_gen(5), device="cuda").to(DTYPES[M % 3])
+    z = fa.int8_matmul(a, sa, b, sb, bias=bias, out_dtype=dtype)
+    _check(z, acc, sa, sb, bias)
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_matmul_at_the_largest_sums(M):
+    """K at its limit and every product 2^14: the int32 sums do not wrap."""
+    K = 131071
+    a = torch.full((M, K), -128, dtype=torch.int8, device="cuda")
+    b = torch.full((33, K), -128, dtype=torch.int8, device="cuda")
+    b[1::2] = 127
+    one = torch.ones(M, device="cuda"), torch.ones(33, device="cuda")
+    y = fa.int8_matmul(a, one[0], b, one[1], out_dtype=torch.float32)
+    want = torch.full((M, 33), float(K * 16384), device="cuda")
+    want[:, 1::2] = float(-K * 128 * 127)
+    assert torch.equal(y, want)
+    with pytest.raises(ValueError, match="131071"):
+        fa.int8_matmul(torch.zeros(1, K + 1, dtype=torch.int8, device="cuda"), one[0][:1],
+                       torch.zeros(1, K + 1, dtype=torch.int8, device="cuda"), one[1][:1])
+
+
+@pytest.mark.parametrize("M", [1, 20, 150, 700])
+def test_matmul_strides_and_alignment(M):
+    N, K = 200, 512
+    big_a, big_b = _ints((M, 700), 1), _ints((N, 800), 2)
+    sa, sb = _scales(2 * M, 3), _scales(2 * N, 4)
+    for oa, ob in ((0, 0), (16, 32), (1, 0), (0, 3), (8, 8)):
+        a, b = big_a[:, oa:oa + K], big_b[:, ob:ob + K]
+        y = fa.int8_matmul(a, sa[::2], b, sb[1::2])
+        assert torch.equal(y, fa.int8_matmul(a.contiguous(), sa[::2].contiguous(), b.contiguous(),
+                                             sb[1::2].contiguous()))
+        _check(y, _exact(a, b), sa[::2], sb[1::2])
+    assert torch.equal(fa.int8_matmul(a.t().contiguous().t(), sa[::2], b, sb[1::2]), y)
+    one = big_a[:1, :K].expand(M, K)
+    _check(fa.int8_matmul(one, sa[:M], b, sb[:N]), _exact(one, b), sa[:M], sb[:N])
+    for pad in (8, 3):  # a destination inside a wider one
+        buf = torch.full((M, N + 2 * pad), 5.0, dtype=torch.bfloat16, device="cuda")
+        out = fa.int8_matmul(a, sa[::2], b, sb[1::2], out=buf[:, pad:pad + N])
+        assert torch.equal(out, y) and torch.equal(buf[:, pad:pad + N], y)
+        assert bool((buf[:, :pad] == 5).all()) and bool((buf[:, pad + N:] == 5).all())
+
+
+# rows of each expert, tokens (0: rows of a directly), N, K, spare rows behind the last
+GROUPS = [([1], 0, 64, 128, 0), ([0, 0, 3], 0, 16, 64, 2), ([5, 0, 1, 0, 64, 65], 0, 130, 272, 7),
+          ([1] * 40, 13, 256, 1024, 8), ([2, 0, 5, 1] * 8, 64, 4096, 2048, 100), ([0] * 5, 4, 64, 64, 9),
+          ([300, 0, 17, 129, 256, 1], 500, 512, 640, 30), ([257], 100, 300, 1040, 1), ([1000, 3, 500], 0, 768, 2048, 0),
+          ([0, 2500, 0, 40], 1024, 1024, 512, 64), ([3] * 1024, 0, 33, 48, 1), ([70] * 32, 300, 512, 1536, 5)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("case", GROUPS, ids=lambda c: f"{len(c[0])}x{sum(c[0])}-{c[1]}-{c[2]}-{c[3]}")
+def test_grouped(case, dtype):
+    counts, tokens, N, K, spare = case
+    E, R = len(counts), sum(counts) + spare
+    offs = torch.tensor([0] + counts).cumsum(0).to(torch.int32).cuda()
+    M = tokens or R
+    a, b, sa, sb = _ints((M, K), 1), _ints((E, N, K), 2), _scales(M, 3), _scales((E, N), 4)
+    ids = torch.randint(0, M, (R,), generator=_gen(5), device="cuda", dtype=torch.int32) if tokens else None
+    if tokens:
+        ids[sum(counts):] = -1  # not read
+    y = fa.int8_grouped_matmul(a, sa, b, sb, offs, row_ids=ids, out_dtype=dtype)
+    assert y.shape == (R, N) and not y[sum(counts):].any()
+    lo = 0
+    for e, c in enumerate(counts):
+        if c:
+            src = ids[lo:lo + c].long() if tokens else slice(lo, lo + c)
+            _check(y[lo:lo + c], _exact(a[src], b[e]), sa[src], sb[e])
+        lo += c
+    buf = torch.full((R, N), 9.0, dtype=dtype, device="cuda")
+    fa.int8_grouped_matmul(a, sa, b, sb, offs, row_ids=ids, out=buf)
+    assert torch.equal(buf[:lo], y[:lo]) and bool((buf[lo:] == 9).all())
+
+
+@pytest.mark.parametrize("K", [512, 515])
+@pytest.mark.parametrize("rows", [30, 400])
+def test_grouped_strided_weights_and_bad_ids(rows, K):
+    E, N, M = 3, 96, 50
+    w = _ints((E, N + 8, K + 16), 1)[:, 4:4 + N, :K]
+    a, sa, sb = _ints((M, K), 2), _scales(M, 3), _scales((E, N), 4)
+    offs = torch.tensor([0, rows // 3, rows // 2, rows], dtype=torch.int32, device="cuda")
+    ids = torch.randint(0, M, (rows,), generator=_gen(5), device="cuda", dtype=torch.int32)
+    good = fa.int8_grouped_matmul(a, sa, w.contiguous(), sb, offs, row_ids=ids)
+    assert torch.equal(fa.int8_grouped_matmul(a, sa, w, sb, offs, row_ids=ids), good)
+    ids[::7] = M
+    ids[3] = -5
+    y = fa.int8_grouped_matmul(a, sa, w, sb, offs, row_ids=ids)
+    out = (ids < 0) | (ids >= M)
+    assert bool(torch.isnan(y[out]).all()) and torch.equal(y[~out], good[~out])
+    # offsets past the rows are cut to them
+    far = torch.tensor([0, rows // 3, rows // 2, 1 << 30], dtype=torch.int32, device="cuda")
+    assert torch.equal(fa.int8_grouped_matmul(a, sa, w, sb, far, row_ids=ids)[~out], good[~out])
+
+
+QUANT = [(1, 1), (1, 7168), (3, 7), (5, 1024), (64, 1025), (33, 2048), (7, 4100), (100, 8192), (2, 40000), (4096, 64)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", QUANT, ids=str)
+def test_quantize_is_the_formula(shape, dtype):
+    M, K = shape
+    x = (torch.randn(M, K, generator=_gen(1), device="cuda") * torch.logspace(-3, 3, M, device="cuda")[:, None]).to(dtype)
+    x[M // 2] = 0
+    q, s = fa.quantize_int8(x)
+    xc = x.cpu().float()
+    want_s = xc.abs().amax(dim=1).clamp_min(1e-10) / 127.0
+    assert torch.equal(s.cpu(), want_s)
+    assert torch.equal(q.cpu(), torch.round(xc / want_s[:, None]).to(torch.int8))
+    # rows at a distance, and odd ones
+    wide = torch.zeros(M, K + 5, dtype=dtype, device="cuda")
+    wide[:, 5:] = x
+    q2, s2 = fa.quantize_int8(wide[:, 5:])
+    assert torch.equal(q2, q) and torch.equal(s2, s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", QUANT, ids=str)
+def test_swiglu_quantize(shape, dtype):
+    M, K = shape
+    x = torch.randn(M, 2 * K, generator=_gen(2), device="cuda").mul_(3).to(dtype)
+    q, s = fa.swiglu_quantize_int8(x)
+    v = x.to(F64)
+    v = v[:, K:] * torch.sigmoid(v[:, K:]) * v[:, :K]
+    want = v.abs().amax(dim=1).clamp_min(1e-10) / 127.0
+    # exp within 2 steps (4 U), then sum, quotient and product (3 U), the scale's quotient (1 U)
+    assert bool(((s.to(F64) - want).abs() <= 8 * U * want * 1.001).all())
+    # q is rint of a quotient that is within 7 + 8 + 1 U of the exact one
+    assert bool(((q.to(F64) - v / want[:, None]).abs() <= 0.5 + 127 * 16.1 * U).all())
+
+
+def test_quantize_rows_in_use_and_poisoned_rows():
+    x = torch.randn(10, 96, generator=_gen(1), device="cuda")
+    n = torch.tensor([6], dtype=torch.int32, device="cuda")
+    q0, s0 = fa.quantize_int8(x)
+    q, s = fa.quantize_int8(x, num_rows=n)
+    assert torch.equal(q[:6], q0[:6]) and torch.equal(s[:6], s0[:6]) and not q[6:].any() and not s[6:].any()
+    qb, sb = torch.full_like(q, 5), torch.full_like(s, 5.0)
+    fa.quantize_int8(x, num_rows=n, q=qb, scale=sb)
+    assert torch.equal(qb[:6], q0[:6]) and bool((qb[6:] == 5).all()) and bool((sb[6:] == 5).all())
+    x[2, 50], x[4, 0] = float("nan"), float("-inf")
+    q, s = fa.quantize_int8(x)
+    y = fa.int8_matmul(q, s, _ints((16, 96), 3), torch.ones(16, device="cuda"))
+    bad = torch.tensor([2, 4], device="cuda")
+    assert bool(torch.isnan(y[bad]).all())
+    keep = [i for i in range(10) if i not in (2, 4)]
+    assert bool(torch.isfinite(y[keep]).all()) and torch.equal(q[keep], q0[keep])
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 outputs, and weights of more than 2^31 bytes."""
+    M, N, K = 70000, 32768, 32
+    a, b, sa, sb = _ints((M, K), 1), _ints((N, K), 2), _scales(M, 3), _scales(N, 4)
+    y = fa.int8_matmul(a, sa, b, sb)
+    _check(y[-300:], _exact(a[-300:], b), sa[-300:], sb)
+    del y
+    E, N, K = 3, 16384, 65536
+    w = torch.zeros(E, N, K, dtype=torch.int8, device="cuda")
+    w[2] = _ints((N, K), 5)
+    offs = torch.tensor([0, 1, 2, 40], dtype=torch.int32, device="cuda")
+    a, sa, sb = _ints((40, K), 6), _scales(40, 7), _scales((E, N), 8)
+    y = fa.int8_grouped_matmul(a, sa, w, sb, offs)
+    _check(y[2:, -200:], _exact(a[2:], w[2, -200:]), sa[2:], sb[2, -200:])
+    assert not y[:2].any()
+
+
+@pytest.mark.parametrize("T", [1, 3, 40, 700])
+def test_expert_layer_in_int8(T):
+    """route, sort, gathered product, SwiGLU and quantiser, second product,
+    and back: against the same layer in 64 bits, quantised at the same places."""
+    from flashinfer_amd import kernel
+    H, I, E, off = 1024, 512, 32, 64
+    g = _gen(T)
+    logits = torch.randn(T, 256, generator=g, device="cuda")
+    logits[:, off:off + E] += 1.5
+    ids, w = kernel.route(logits, torch.zeros(256, device="cuda"), 2.5)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    w1, w2 = _ints((E, 2 * I, H), 1), _ints((E, H, I), 2)
+    s1, s2 = _scales((E, 2 * I), 3), _scales((E, H), 4)
+
+    def layer():
+        plan = fa.sort_experts(ids, E, off)
+        q, s = fa.quantize_int8(x)
+        h = fa.int8_grouped_matmul(q, s, w1, s1, plan.expert_offsets, row_ids=plan.token_of_row)
+        q, s = fa.swiglu_quantize_int8(h, num_rows=plan.expert_offsets[-1:])
+        return plan, h, q, s, fa.unpermute(fa.int8_grouped_matmul(q, s, w2, s2, plan.expert_offsets), plan, w)
+
+    plan, h, q, s, y = layer()
+    S = int(plan.expert_offsets[-1])
+    ref = torch.zeros(T, H, dtype=F64, device="cuda")
+    qx, sx = fa.quantize_int8(x)
+    for t in range(T) if T <= 40 else (0, 1, T // 2, T - 1):
+        for j in range(8):
+            e = int(ids[t, j]) - off
+            if 0 <= e < E:
+                p = int(plan.row_of_slot[t, j])
+                assert p < S
+                _check(h[p:p + 1], _exact(qx[t:t + 1], w1[e]), sx[t:t + 1], s1[e])
+                row = (_exact(q[p:p + 1], w2[e]) * s[p].to(F64) * s2[e].to(F64))[0]
+                ref[t] += float(w[t, j]) * row
+    # bf16 rows (2^-8 of each term), summed in fp32, rounded once more
+    rows = [t for t in (range(T) if T <= 40 else (0, 1, T // 2, T - 1))]
+    size = torch.zeros_like(ref)
+    for t in rows:
+        for j in range(8):
+            e = int(ids[t, j]) - off
+            if 0 <= e < E:
+                p = int(plan.row_of_slot[t, j])
+                size[t] += abs(float(w[t, j])) * (_exact(q[p:p + 1], w2[e]) * s[p].to(F64) * s2[e].to(F64))[0].abs()
+    bound = size * (2.0 ** -8 + 16 * U) * 1.01 + ref.abs() * 2.0 ** -8
+    assert bool(((y[rows].to(F64) - ref[rows]).abs() <= bound[rows]).all())
+    # captured and replayed
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        layer()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        *_, z = layer()
+    for rep in range(3):
+        x.copy_(torch.randn(T, H, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(z, layer()[-1])
+
+
+def test_two_streams_and_threads():
+    import threading
+    a, b, sa, sb = _ints((200, 2048), 1), _ints((1024, 2048), 2), _scales(200, 3), _scales(1024, 4)
+    want = fa.int8_matmul(a, sa, b, sb)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                got = [fa.int8_matmul(a[:m], sa[:m], b, sb) for m in (1, 16, 64, 200)]
+            st.synchronize()
+        bad.extend(0 for y in got if not torch.equal(y, want[:len(y)]))
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_refusals():
+    a, b = _ints((4, 32), 1), _ints((8, 32), 2)
+    sa, sb = _scales(4, 3), _scales(8, 4)
+    w, sw = _ints((2, 8, 32), 2), _scales((2, 8), 4)
+    offs = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    out = torch.zeros(4, 8, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(4, 32, device="cuda")
+    bad = [
+        (TypeError, lambda: fa.int8_matmul(a.float(), sa, b, sb)),
+        (TypeError, lambda: fa.int8_matmul(a, sa, b.view(torch.uint8), sb)),
+        (TypeError, lambda: fa.int8_matmul(a, sa.half(), b, sb)),
+        (TypeError, lambda: fa.int8_matmul(a, sa, b, sb, out_dtype=torch.float64)),
+        (TypeError, lambda: fa.int8_matmul(a, sa, b, sb, bias=torch.zeros(8, device="cuda", dtype=torch.float64))),
+        (ValueError, lambda: fa.int8_matmul(a[:, :16], sa, b, sb)),
+        (ValueError, lambda: fa.int8_matmul(a, sa[:3], b, sb)),
+        (ValueError, lambda: fa.int8_matmul(a, sa[:, None], b, sb)),
+        (ValueError, lambda: fa.int8_matmul(a, sa, b, sb, bias=torch.zeros(1, device="cuda"))),
+        (ValueError, lambda: fa.int8_matmul(a, sa, b.cpu(), sb)),
+        (ValueError, lambda: fa.int8_matmul(a.cpu(), sa, b, sb)),
+        (ValueError, lambda: fa.int8_matmul(a, sa, b, sb, out=out[:3])),
+        (ValueError, lambda: fa.int8_matmul(a, sa, b, sb, out=out[:1].expand(4, 8))),
+        (ValueError, lambda: fa.int8_matmul(a, sa, b, sb.clone().requires_grad_())),
+        (ValueError, lambda: fa.int8_matmul(a[:, :0], sa, b[:, :0], sb)),
+        (ValueError, lambda: fa.int8_grouped_matmul(a, sa, b, sb, offs)),
+        (ValueError, lambda: fa.int8_grouped_matmul(a, sa, w, sw, offs[:2])),
+        (TypeError, lambda: fa.int8_grouped_matmul(a, sa, w, sw, offs.long())),
+        (TypeError, lambda: fa.int8_grouped_matmul(a, sa, w, sw, offs, row_ids=offs.long())),
+        (ValueError, lambda: fa.int8_grouped_matmul(a, sa, w, sw[0], offs)),
+        (TypeError, lambda: fa.quantize_int8(x.double())),
+        (ValueError, lambda: fa.quantize_int8(x[0])),
+        (ValueError, lambda: fa.quantize_int8(x.clone().requires_grad_())),
+        (ValueError, lambda: fa.swiglu_quantize_int8(x[:, :31])),
+        (TypeError, lambda: fa.quantize_int8(x, num_rows=torch.zeros(1, device="cuda"))),
+        (ValueError, lambda: fa.quantize_int8(x, num_rows=offs)),
+        (TypeError, lambda: fa.quantize_int8(x, q=x)),
+        (ValueError, lambda: fa.quantize_int8(x, scale=sa[:2])),
+    ]
+    for n, (error, call) in enumerate(bad):
+        with pytest.raises(error):
+            call()
+            print("not refused:", n)
+    assert fa.int8_matmul(a[:0], sa[:0], b, sb).shape == (0, 8)
+    assert fa.int8_matmul(a, sa, b[:0], sb[:0]).shape == (4, 0)
+    assert fa.int8_grouped_matmul(a[:0], sa[:0], w, sw, offs * 0).shape == (0, 8)
+    q, s = fa.quantize_int8(x[:0])
+    assert q.shape == (0, 32) and s.shape == (0,)
