@@ -30,7 +30,8 @@ SOURCES = ["route.hip", "sort.hip", "gemm1.hip", "gemm2.hip", "gemm1_tile.hip", 
            "gemm1_wide.hip", "gemm2_wide.hip", "gemm2_combine.hip", "combine.hip", "quant.hip", "capi.hip"]
 # operators whose sizes are arguments: one library for all definitions
 EXPERTS_LIB = os.path.join(HERE, "libmi_experts.so")
-EXPERTS_SOURCES = ["experts_sort.hip", "experts_move.hip", "int8_quant.hip", "int8_gemm.hip",
+EXPERTS_SOURCES = ["experts_sort.hip", "experts_move.hip", "int8_quant.hip", "int8_gemm.hip", "int8_any.hip",
+                   "int8_tile.hip", "int8_wide.hip",
                    "experts_capi.hip"]
 PEAKS_LIB = os.path.join(HERE, "libmi_peaks.so")
 PEAKS_SOURCES = ["peaks.hip"]

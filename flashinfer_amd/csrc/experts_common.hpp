@@ -48,6 +48,8 @@ __device__ __forceinline__ void store(T* p, const float (&v)[N]) {
     }
 }
 
+template <int N> struct IntC { static constexpr int value = N; };
+
 // Launchers (host).
 hipError_t launch_sort(const int32_t* ids, int64_t T, int k, int E, int64_t offset, int32_t* offsets,
                        int32_t* token_of_row, int32_t* row_of_slot, int32_t* counts, hipStream_t s);

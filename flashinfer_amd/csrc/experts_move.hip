@@ -200,8 +200,6 @@ __global__ __launch_bounds__(THREADS) void unpermute_backward_kernel(
 
 // Calls go(T{}, IntC<N>{}) with the widest vector (16 bytes, else 1 element)
 // that the row length, strides (in elements) and addresses allow.
-template <int N> struct IntC { static constexpr int value = N; };
-
 template <class F>
 hipError_t by_type(int dtype, uint64_t elems, uint64_t addresses, F go) {
     const int size = dtype == MI_EXPERTS_F32 ? 4 : 2;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "experts_common.hpp"
+#include "lds_copy.hpp"
 
 namespace miexp {
 
@@ -35,48 +36,96 @@ __device__ __forceinline__ int64_t clamped(const int32_t* offsets, int e, int64_
     return max((int64_t)0, min((int64_t)offsets[e], rows));
 }
 
-// Row tile `mt` of BM rows: its expert, first row and rows. Experts have
-// ceil(rows / BM) tiles each, in order; a wave looks at 64 of them at a time.
-// False past the last tile. Uniform over the workgroup.
+// The experts' row tiles of BM rows, in order: ceil(rows / BM) of each. A wave
+// looks at 64 experts at a time. Uniform over the workgroup.
+struct Tiles {
+    int e, first;   // expert, and its first row tile
+    int tiles;      // its row tiles
+    int row, end;   // its rows
+};
+
+// Row tiles of lane's expert e0 + lane (none past the last), and their inclusive sum.
 template <int BM>
-__device__ __forceinline__ bool find_tile(const Int8Call& p, int64_t mt, int& e, int64_t& row0, int& nrows) {
-    if (!p.offsets) {
-        e = 0;
-        row0 = mt * BM;
-        if (row0 >= p.rows) return false;
-        nrows = (int)min((int64_t)BM, p.rows - row0);
-        return true;
+__device__ __forceinline__ int scan_tiles(const Int8Call& p, int e0, int& lo, int& hi, int& inc) {
+    const int lane = threadIdx.x & 63, x = e0 + lane;
+    lo = hi = 0;
+    if (x < p.E) {
+        lo = (int)clamped(p.offsets, x, p.rows);
+        hi = max(lo, (int)clamped(p.offsets, x + 1, p.rows));
     }
-    const int lane = threadIdx.x & 63;
-    int64_t before = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 64) {
-        const int x = e0 + lane;
-        int64_t lo = 0, hi = 0;
-        if (x < p.E) {
-            lo = clamped(p.offsets, x, p.rows);
-            hi = max(lo, clamped(p.offsets, x + 1, p.rows));
-        }
-        const int tiles = (int)((hi - lo + BM - 1) / BM);
-        int inc = tiles;
+    const int tiles = (hi - lo + BM - 1) / BM;
+    inc = tiles;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int u = __shfl_up(inc, d);
-            if (lane >= d) inc += u;
-        }
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(inc, d);
+        if (lane >= d) inc += u;
+    }
+    return tiles;
+}
+
+// The expert that has row tile mt. False past the last tile.
+template <int BM>
+__device__ __forceinline__ bool find_expert(const Int8Call& p, int mt, Tiles& t) {
+    if (!p.offsets) {
+        t = Tiles{0, 0, (int)((p.rows + BM - 1) / BM), 0, (int)p.rows};
+        return mt < t.tiles;
+    }
+    int before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 64) {
+        int lo, hi, inc;
+        const int tiles = scan_tiles<BM>(p, e0, lo, hi, inc);
         const unsigned long long has = __ballot(before + inc > mt);
         if (has) {
             const int l = __ffsll(has) - 1;
-            e = __builtin_amdgcn_readfirstlane(e0 + l);
-            const int at = __builtin_amdgcn_readfirstlane(__shfl(inc - tiles, l));
-            const int first = __builtin_amdgcn_readfirstlane(__shfl((int)lo, l));
-            const int end = __builtin_amdgcn_readfirstlane(__shfl((int)hi, l));
-            row0 = first + (mt - before - at) * BM;
-            nrows = (int)min((int64_t)BM, end - row0);
+            t.e = __builtin_amdgcn_readfirstlane(e0 + l);
+            t.first = __builtin_amdgcn_readfirstlane(before + __shfl(inc - tiles, l));
+            t.tiles = __builtin_amdgcn_readfirstlane(__shfl(tiles, l));
+            t.row = __builtin_amdgcn_readfirstlane(__shfl(lo, l));
+            t.end = __builtin_amdgcn_readfirstlane(__shfl(hi, l));
             return true;
         }
-        before += __shfl(inc, 63);
+        before += __builtin_amdgcn_readfirstlane(__shfl(inc, 63));
     }
     return false;
+}
+
+// Row tile mt: its expert, first row and rows.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const Int8Call& p, int mt, int& e, int64_t& row0, int& nrows) {
+    Tiles t;
+    if (!find_expert<BM>(p, mt, t)) return false;
+    e = t.e;
+    row0 = (int64_t)t.row + (int64_t)(mt - t.first) * BM;
+    nrows = (int)min((int64_t)BM, t.end - row0);
+    return true;
+}
+
+template <int BM>
+__device__ __forceinline__ int count_tiles(const Int8Call& p) {
+    if (!p.offsets) return (int)((p.rows + BM - 1) / BM);
+    int total = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 64) {
+        int lo, hi, inc;
+        scan_tiles<BM>(p, e0, lo, hi, inc);
+        total += __builtin_amdgcn_readfirstlane(__shfl(inc, 63));
+    }
+    return total;
+}
+
+// Tile t of `total` in an order in which tiles that run at the same time share
+// operands: an expert's row tiles go in groups of GM, channel tiles inside a
+// group, row tiles innermost.
+template <int BM, int GM>
+__device__ __forceinline__ void tile_at(const Int8Call& p, int t, int ntiles, int& e, int64_t& row0, int& nrows,
+                                        int& nt) {
+    Tiles x;
+    find_expert<BM>(p, t / ntiles, x);
+    const int u = t - x.first * ntiles;
+    const int grp = u / (GM * ntiles), gm = min(GM, x.tiles - grp * GM), v = u - grp * GM * ntiles;
+    nt = v / gm;
+    e = x.e;
+    row0 = (int64_t)x.row + (int64_t)(grp * GM + v - nt * gm) * BM;
+    nrows = (int)min((int64_t)BM, x.end - row0);
 }
 
 // Row of a that feeds row m of the product; -1 for an id that is none.
@@ -93,10 +142,112 @@ __device__ __forceinline__ float bias_at(const Int8Call& p, int n) {
     return (float)reinterpret_cast<const __bf16*>(p.bias)[n];
 }
 
+// 16 zero bytes: what copies past the end of K read.
+static __device__ const v4i kZeros = {0, 0, 0, 0};
+static __device__ const float kNan = __builtin_nanf("");  // the scale of a row that is none
+
+__device__ __forceinline__ float row_scale(const Int8Call& p, int64_t row) {
+    const int64_t from = source_row(p, row);
+    return from >= 0 ? p.a_scale[from] : __builtin_nanf("");
+}
+
+// Scales and bias of four neighbouring channels n .. n + 3 of expert e.
+struct Channels {
+    float s[4], b[4];
+    __device__ __forceinline__ Channels(const Int8Call& p, int e, int n) {
+        const float* scale = p.b_scale + (int64_t)e * p.N;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[v] = scale[min(n + v, p.N - 1)];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) b[v] = 0.f;
+        if (p.bias) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) b[v] = bias_at(p, min(n + v, p.N - 1));
+        }
+    }
+};
+
+// The four outputs of a row at out (channels n ..) from their integer sums.
+// vec: rows of out hold aligned groups of four.
+template <class T>
+__device__ __forceinline__ void finish4(T* out, int n, int N, const v4i& acc, float sa, const Channels& c, bool vec) {
+    float y[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) y[v] = (float)acc[v] * sa * c.s[v] + c.b[v];
+    if (vec && n + 4 <= N) {
+        store<T, 4>(out, y);
+        return;
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+        if (n + v < N) out[v] = (T)y[v];
+}
+
+// A wave's MT x NT sums: rows row_at + 16 m + lane % 16 of the tile, channels
+// n_at + 16 n + 4 (lane / 16) ... ACC(m, n) gives the sums.
+template <class T, int MT, int NT, class ACC>
+__device__ __forceinline__ void store_tiles(const Int8Call& p, int e, int64_t row0, int nrows, int row_at, int n_at,
+                                            bool vec, ACC acc) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    float sa[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = row_at + m * 16 + r;
+        sa[m] = row < nrows ? row_scale(p, row0 + row) : 0.f;
+    }
+    T* out = reinterpret_cast<T*>(p.out) + (row0 + row_at + r) * p.out_stride;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int at = n_at + n * 16 + 4 * g;
+        if (at >= p.N) break;
+        const Channels c(p, e, at);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            if (row_at + m * 16 + r < nrows)
+                finish4<T>(out + m * 16 * p.out_stride + at, at, p.N, acc(m, n), sa[m], c, vec);
+    }
+}
+
+// Sums of the KS groups of four waves that shared K, in group 0. smem: the
+// whole workgroup's, free once all are here.
+template <int KS, int MT, int NT>
+__device__ __forceinline__ void sum_groups(uint8_t* smem, int ks, int wave, v4i (&acc)[MT][NT]) {
+    if constexpr (KS > 1) {
+        __syncthreads();
+        v4i* sum = reinterpret_cast<v4i*>(smem) + (wave * 64 + (threadIdx.x & 63));
+        if (ks > 0) {
+#pragma unroll
+            for (int i = 0; i < MT * NT; ++i) sum[((ks - 1) * MT * NT + i) * 256] = acc[i / NT][i % NT];
+        }
+        __syncthreads();
+        if (ks > 0) return;
+#pragma unroll
+        for (int i = 0; i < MT * NT; ++i)
+#pragma unroll
+            for (int k = 0; k < KS - 1; ++k) acc[i / NT][i % NT] += sum[(k * MT * NT + i) * 256];
+    }
+}
+
 // Upper bound of row tiles: a tile each for the full ones, one more per expert.
 inline int64_t max_tiles(int64_t rows, int bm, int E) {
     const int64_t full = (rows + bm - 1) / bm;
     return E ? (rows / bm + (rows < E ? rows : E)) : full;
+}
+
+// Kernels for any operands, and for those whose strides and addresses are
+// multiples of 16.
+bool int8_offsets_fit(const Int8Call& p, int bm, int bn);  // a tile's lane offsets within 32 bits
+enum class Int8Tile { T32x32, T32x64, T64x64_K2, T64x64, T64x128_K2, T64x128, T128x128_K2, T128x128, T256x256 };
+hipError_t launch_int8_any(const Int8Call& p, int out_dtype, Int8Tile tile, bool vec, hipStream_t s);
+hipError_t launch_int8_tile(const Int8Call& p, int out_dtype, Int8Tile tile, bool vec, hipStream_t s);
+hipError_t launch_int8_wide(const Int8Call& p, int out_dtype, hipStream_t s);
+
+// Calls f(T{}) with the float type of MI_EXPERTS_* dtype.
+template <class F>
+hipError_t by_out_type(int dtype, F f) {
+    if (dtype == MI_EXPERTS_F32) return f(float{});
+    if (dtype == MI_EXPERTS_F16) return f(_Float16{});
+    return f(__bf16{});
 }
 
 }  // namespace miexp

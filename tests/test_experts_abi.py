@@ -117,7 +117,7 @@ def test_int8_matmul_refuses():
             (good, dict(out_dtype=5), "dtype"), (good, dict(bias=P, bias_dtype=5), "dtype"),
             (good, dict(reserved=1), "reserved"), (good, dict(row_ids=P), "grouped"),
             (good, dict(expert_offsets=P), "grouped"), (good, dict(num_experts=-1), "num_experts"),
-            (good, dict(N=1 << 30, rows=1 << 20, a_rows=1 << 20, out_stride=1 << 30), "too many"),
+            (good, dict(N=1 << 29, rows=1 << 20, a_rows=1 << 20, out_stride=1 << 29), "too many"),
             (good, dict(a_rows=-1, rows=-1), "size"), (grouped, dict(expert_offsets=None), "NULL"),
             (grouped, dict(bias=P), "bias"), (grouped, dict(num_experts=1025), "num_experts")]:
         a = Args(**dict(base, **change))

@@ -135,6 +135,30 @@ def test_grouped(case, dtype):
     assert torch.equal(buf[:lo], y[:lo]) and bool((buf[lo:] == 9).all())
 
 
+# the tiles of csrc/int8_common.hpp, each at sizes that end inside it
+@pytest.mark.parametrize("tile", range(9))
+@pytest.mark.parametrize("shape", [(1, 8, 144), (70, 90, 272), (130, 264, 2048), (259, 515, 1040), (300, 40, 7),
+                                   (520, 700, 1111), (1030, 1000, 128)], ids=str)
+def test_every_tile(tile, shape, monkeypatch):
+    monkeypatch.setenv("MI_INT8_TILE", str(tile))
+    M, N, K = shape
+    a, b, sa, sb = _ints((M, K), 1), _ints((4, N, K), 2), _scales(M, 3), _scales((4, N), 4)
+    bias = torch.randn(N, generator=_gen(5), device="cuda")
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(fa.int8_matmul(a, sa, b[1], sb[1], bias=bias, out_dtype=dtype), _exact(a, b[1]), sa, sb[1], bias)
+    # experts whose rows end inside, at and behind a tile's end, one without rows
+    ends = [0, M // 7, M // 7, M // 7 + min(128, M // 2), M]
+    offs = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(M, generator=_gen(6), device="cuda").to(torch.int32)
+    for rows in (None, ids):
+        y = fa.int8_grouped_matmul(a, sa, b, sb, offs, row_ids=rows)
+        for e in range(4):
+            at = torch.arange(ends[e], ends[e + 1], device="cuda")
+            src = at if rows is None else ids[at].long()
+            if len(at):
+                _check(y[at], _exact(a[src], b[e]), sa[src], sb[e])
+
+
 @pytest.mark.parametrize("K", [512, 515])
 @pytest.mark.parametrize("rows", [30, 400])
 def test_grouped_strided_weights_and_bad_ids(rows, K):
