@@ -24,7 +24,7 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 bool float_type(int32_t d) { return d == MI_EXPERTS_BF16 || d == MI_EXPERTS_F32 || d == MI_EXPERTS_F16; }
 size_t size_of(int32_t d) { return d == MI_EXPERTS_F32 ? 4 : 2; }
 
-// The row-moving kernels put column chunks of at least 256 units in grid.y.
+// Rows of the row-moving kernels: at most 2^15 chunks of 256 units.
 constexpr int64_t MAX_ROW_BYTES = 1 << 23;
 
 int hip_status(const char* who, hipError_t e) {

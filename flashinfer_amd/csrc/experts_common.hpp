@@ -26,6 +26,12 @@ template <class T, int N> struct Vec { typedef T type __attribute__((ext_vector_
 template <class T> struct Vec<T, 1> { typedef T type; };
 
 template <class T, int N>
+__device__ __forceinline__ float element(const typename Vec<T, N>::type& v, int i) {
+    if constexpr (N == 1) return (float)v;
+    else return (float)v[i];
+}
+
+template <class T, int N>
 __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
     if constexpr (N == 1) {
         v[0] = (float)*p;

@@ -8,7 +8,9 @@
 // fp32 in a fixed order; no atomics. All are bound by HBM.
 //
 // tx = 2^tx_log lanes share a token (as many as its row has vectors, at most
-// a workgroup), so short rows still fill the waves.
+// a workgroup), so short rows still fill the waves. From 64 lanes on a wave has
+// one token (ONE): its places, weights and whether a slot is local are then
+// scalar, and slots of other shards cost a scalar branch.
 #include "experts_common.hpp"
 
 namespace miexp {
@@ -22,13 +24,31 @@ inline int lanes_log(int64_t vectors) {
     return l;
 }
 
+// The token of this thread in a group of THREADS >> tx_log.
+template <bool ONE>
+__device__ __forceinline__ int token_in_group(int tx_log) {
+    const int t = threadIdx.x >> tx_log;
+    return ONE ? __builtin_amdgcn_readfirstlane(t) : t;
+}
+
 inline unsigned blocks_for(int64_t T, int tx_log) {
     const int64_t b = (T + (THREADS >> tx_log) - 1) / (THREADS >> tx_log);
     return (unsigned)(b < MAX_BLOCKS ? b : MAX_BLOCKS);
 }
 
+// Rows of slots j0 .. j0 + KG - 1 of token t (-1 past the k of it), all loaded
+// before the first is used: loads and stores of rows in between would be
+// waited for with them, memory operations completing in order.
+__device__ __forceinline__ void rows_of(const int32_t* row_of_slot, int64_t t, int k, int j0, int (&row)[KG]) {
+#pragma unroll
+    for (int j = 0; j < KG; ++j) row[j] = row_of_slot[t * k + min(j0 + j, k - 1)];
+#pragma unroll
+    for (int j = 0; j < KG; ++j)
+        if (j0 + j >= k) row[j] = -1;
+}
+
 // V: the unit that moves, as wide as row length, strides and addresses allow.
-template <class V>
+template <class V, bool ONE>
 __global__ __launch_bounds__(THREADS) void permute_kernel(const char* __restrict__ x, int64_t x_stride,
                                                           int64_t T, int k, int64_t vectors,
                                                           const int32_t* __restrict__ row_of_slot,
@@ -40,15 +60,19 @@ __global__ __launch_bounds__(THREADS) void permute_kernel(const char* __restrict
     const int64_t local = min((int64_t)*num_rows, R);
     const int64_t v = (int64_t)blockIdx.y * tx + (threadIdx.x & (tx - 1));
     if (v >= vectors) return;
-    for (int64_t t = (int64_t)blockIdx.x * (THREADS >> tx_log) + (threadIdx.x >> tx_log); t < T;
+    for (int64_t t = (int64_t)blockIdx.x * (THREADS >> tx_log) + token_in_group<ONE>(tx_log); t < T;
          t += (int64_t)gridDim.x * (THREADS >> tx_log)) {
         const V val = reinterpret_cast<const V*>(x + t * x_stride)[v];
-        for (int j = 0; j < k; ++j) {
-            const int64_t row = row_of_slot[t * k + j];
-            if (row >= 0 && row < local)
-                reinterpret_cast<V*>(rows + row * rows_stride)[v] = val;
-            else if (zero_rest && row >= 0 && row < R)
-                reinterpret_cast<V*>(rows + row * rows_stride)[v] = V{};
+        for (int j0 = 0; j0 < k; j0 += KG) {
+            int row[KG];
+            rows_of(row_of_slot, t, k, j0, row);
+#pragma unroll
+            for (int j = 0; j < KG; ++j) {
+                if (row[j] >= 0 && row[j] < local)
+                    reinterpret_cast<V*>(rows + row[j] * rows_stride)[v] = val;
+                else if (zero_rest && row[j] >= 0 && row[j] < R)
+                    reinterpret_cast<V*>(rows + row[j] * rows_stride)[v] = V{};
+            }
         }
     }
 }
@@ -63,8 +87,9 @@ hipError_t launch_permute(const void* x, int64_t x_stride, int64_t T, int k, int
         const int64_t vectors = row_bytes / (int64_t)sizeof(V);
         const int tx_log = lanes_log(vectors);
         const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
-        hipLaunchKernelGGL((permute_kernel<V>), grid, dim3(THREADS), 0, s, (const char*)x, x_stride, T, k,
-                           vectors, row_of_slot, num_rows, (char*)rows, rows_stride, (int)zero_rest, tx_log);
+        const auto kernel = tx_log >= 6 ? permute_kernel<V, true> : permute_kernel<V, false>;
+        hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, s, (const char*)x, x_stride, T, k, vectors, row_of_slot,
+                           num_rows, (char*)rows, rows_stride, (int)zero_rest, tx_log);
         return hipGetLastError();
     };
     if (bits % 16 == 0) return go(v4i{});
@@ -74,7 +99,7 @@ hipError_t launch_permute(const void* x, int64_t x_stride, int64_t T, int k, int
     return go((uint8_t)0);
 }
 
-template <class T, int N, bool WEIGHTED>
+template <class T, int N, bool WEIGHTED, bool ONE>
 __global__ __launch_bounds__(THREADS) void unpermute_kernel(const T* __restrict__ rows, int64_t rows_stride,
                                                             int64_t tokens, int k, int64_t H,
                                                             const int32_t* __restrict__ row_of_slot,
@@ -86,31 +111,34 @@ __global__ __launch_bounds__(THREADS) void unpermute_kernel(const T* __restrict_
     const int64_t local = min((int64_t)*num_rows, tokens * k);
     const int64_t c = ((int64_t)blockIdx.y * tx + (threadIdx.x & (tx - 1))) * N;
     if (c >= H) return;
-    for (int64_t t = (int64_t)blockIdx.x * (THREADS >> tx_log) + (threadIdx.x >> tx_log); t < tokens;
+    for (int64_t t = (int64_t)blockIdx.x * (THREADS >> tx_log) + token_in_group<ONE>(tx_log); t < tokens;
          t += (int64_t)gridDim.x * (THREADS >> tx_log)) {
         float acc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.f;
         for (int j0 = 0; j0 < k; j0 += KG) {
-            float v[KG][N], w[KG];
+            int row[KG];
+            float w[KG];
+            rows_of(row_of_slot, t, k, j0, row);
+            if (WEIGHTED) {
+#pragma unroll
+                for (int j = 0; j < KG; ++j) w[j] = weights[t * k + min(j0 + j, k - 1)];
+            }
+            typename Vec<T, N>::type v[KG];
             bool on[KG];
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
-                const bool in = j0 + j < k;
-                const int64_t row = in ? row_of_slot[t * k + j0 + j] : -1;
-                on[j] = row >= 0 && row < local;
-                w[j] = 1.f;
-                if (on[j]) {
-                    load<T, N>(rows + row * rows_stride + c, v[j]);
-                    if (WEIGHTED) w[j] = weights[t * k + j0 + j];
-                }
+                on[j] = row[j] >= 0 && row[j] < local;
+                if (on[j]) v[j] = *reinterpret_cast<const typename Vec<T, N>::type*>(rows + row[j] * rows_stride + c);
             }
 #pragma unroll
             for (int j = 0; j < KG; ++j)
                 if (on[j]) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        acc[i] = WEIGHTED ? fmaf(w[j], v[j][i], acc[i]) : acc[i] + v[j][i];
+                    for (int i = 0; i < N; ++i) {
+                        const float x = element<T, N>(v[j], i);
+                        acc[i] = WEIGHTED ? fmaf(w[j], x, acc[i]) : acc[i] + x;
+                    }
                 }
         }
         store<T, N>(out + t * out_stride + c, acc);
@@ -119,7 +147,7 @@ __global__ __launch_bounds__(THREADS) void unpermute_kernel(const T* __restrict_
 
 // Gradients of a token's rows and weights: its tx lanes walk the columns, each
 // lane keeps one partial product sum per slot, and the sums meet at the end.
-template <class T, int N>
+template <class T, int N, bool ONE>
 __global__ __launch_bounds__(THREADS) void unpermute_backward_kernel(
     const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ rows, int64_t rows_stride,
     int64_t tokens, int k, int64_t H, const int32_t* __restrict__ row_of_slot,
@@ -132,16 +160,16 @@ __global__ __launch_bounds__(THREADS) void unpermute_backward_kernel(
     const int64_t per = THREADS >> tx_log;
     // the same number of rounds for all threads: they meet at the barriers
     for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tokens; t0 += (int64_t)gridDim.x * per) {
-        const int64_t t = t0 + (threadIdx.x >> tx_log);
+        const int64_t t = t0 + token_in_group<ONE>(tx_log);
         const bool live = t < tokens;
         for (int j0 = 0; j0 < k; j0 += KG) {
-            int64_t row[KG];
+            int row[KG];
             float w[KG], dot[KG];
+            rows_of(row_of_slot, min(t, tokens - 1), k, j0, row);
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
-                row[j] = live && j0 + j < k ? row_of_slot[t * k + j0 + j] : -1;
-                if (row[j] >= R) row[j] = -1;
-                w[j] = row[j] >= 0 && weights ? weights[t * k + j0 + j] : 1.f;
+                if (!live || row[j] >= R) row[j] = -1;
+                w[j] = weights ? weights[min(t, tokens - 1) * k + min(j0 + j, k - 1)] : 1.f;
                 dot[j] = 0.f;
             }
             if (live) {
@@ -219,14 +247,10 @@ hipError_t launch_unpermute(int dtype, const void* rows, int64_t rows_stride, in
         const int64_t vectors = (H + N - 1) / N;
         const int tx_log = lanes_log(vectors);
         const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
-        if (weights)
-            hipLaunchKernelGGL((unpermute_kernel<E, N, true>), grid, dim3(THREADS), 0, s, (const E*)rows,
-                               rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)out, out_stride,
-                               tx_log);
-        else
-            hipLaunchKernelGGL((unpermute_kernel<E, N, false>), grid, dim3(THREADS), 0, s, (const E*)rows,
-                               rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)out, out_stride,
-                               tx_log);
+        const auto kernel = weights ? (tx_log >= 6 ? unpermute_kernel<E, N, true, true> : unpermute_kernel<E, N, true, false>)
+                                    : (tx_log >= 6 ? unpermute_kernel<E, N, false, true> : unpermute_kernel<E, N, false, false>);
+        hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, s, (const E*)rows, rows_stride, T, k, H, row_of_slot,
+                           num_rows, weights, (E*)out, out_stride, tx_log);
         return hipGetLastError();
     });
 }
@@ -243,10 +267,10 @@ hipError_t launch_unpermute_backward(int dtype, const void* grad, int64_t grad_s
         typedef decltype(elem) E;
         constexpr int N = decltype(width)::value;
         const int tx_log = lanes_log((H + N - 1) / N);
-        hipLaunchKernelGGL((unpermute_backward_kernel<E, N>), dim3(blocks_for(T, tx_log)), dim3(THREADS), 0,
-                           s, (const E*)grad, grad_stride, (const E*)rows, rows_stride, T, k, H, row_of_slot,
-                           num_rows, weights, (E*)grad_rows, grad_rows_stride, (int)zero_rest, grad_weights,
-                           tx_log);
+        const auto kernel = tx_log >= 6 ? unpermute_backward_kernel<E, N, true> : unpermute_backward_kernel<E, N, false>;
+        hipLaunchKernelGGL(kernel, dim3(blocks_for(T, tx_log)), dim3(THREADS), 0, s, (const E*)grad, grad_stride,
+                           (const E*)rows, rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)grad_rows,
+                           grad_rows_stride, (int)zero_rest, grad_weights, tx_log);
         return hipGetLastError();
     });
 }

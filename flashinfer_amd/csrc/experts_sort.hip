@@ -10,15 +10,14 @@
 // contiguous slots, so the order is that of the slots and no result hangs on
 // the order of atomics.
 //
-// Up to SMALL slots one workgroup does it all (the latency of three passes
-// over LDS). Beyond, one launch counts the buckets of at most 256 chunks, and
-// a second one places them: each workgroup sums the counts of the chunks
-// before its own, which are in L2.
+// Up to SMALL slots one workgroup does it all. Beyond, one launch counts the
+// buckets of at most 256 chunks, and a second one places them: each workgroup
+// sums the counts of the chunks before its own, which are in L2.
 #include "experts_common.hpp"
 
 namespace miexp {
 
-constexpr int64_t SMALL = 8192;
+constexpr int64_t SMALL = 4096;
 constexpr int64_t MAX_CHUNKS = 256;
 constexpr int CHUNK_MIN = 2048;
 
@@ -71,81 +70,100 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
     return before + inc - v;
 }
 
-// Places slots [first, last) whose buckets start at base[b] (b < E + 1 <= 1025,
-// one or two per thread). counts: LDS [waves][E + 1].
-__device__ void place(const int32_t* ids, int64_t first, int64_t last, int k, int E, long long offset,
-                      int bits, int* counts, const int* base, int32_t* token_of_row,
-                      int32_t* row_of_slot) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t per = ((last - first + waves - 1) / waves + 63) / 64 * 64;
-    const int64_t a = first + wave * per, z = min(a + per, last);
-    int* mine = counts + wave * (E + 1);
-    for (int i = threadIdx.x; i < waves * (E + 1); i += blockDim.x) counts[i] = 0;
-    __syncthreads();
-    for (int64_t s = a; s < z; s += 64) {
+// A wave's part of the slots being placed: BATCHES of 64, kept in registers.
+constexpr int BATCHES = 4;
+struct Batch {
+    int bucket;
+    unsigned long long same;  // lanes with this lane's bucket
+};
+
+// Counts the buckets of this wave's slots [a, z) into mine[]; the first
+// BATCHES of them stay in `kept`.
+__device__ __forceinline__ void count_slots(const int32_t* ids, int64_t a, int64_t z, int E, long long offset,
+                                            int bits, int* mine, Batch (&kept)[BATCHES]) {
+    const int lane = threadIdx.x & 63;
+    auto add = [&](int64_t s, int id) {
+        Batch x;
         const bool live = s + lane < z;
-        const int b = live ? bucket_of(ids[s + lane], offset, E) : 0;
-        const unsigned long long m = same_bucket(b, bits, live);
-        if (live && lane == __ffsll(m) - 1) atomicAdd(&mine[b], __popcll(m));
-    }
-    __syncthreads();
-    // counts -> first row of each wave's part of a bucket
-    for (int b = threadIdx.x; b <= E; b += blockDim.x) {
-        int at = base[b];
-        for (int w = 0; w < waves; ++w) {
-            const int c = counts[w * (E + 1) + b];
-            counts[w * (E + 1) + b] = at;
-            at += c;
-        }
-    }
-    __syncthreads();
-    for (int64_t s = a; s < z; s += 64) {
+        x.bucket = live ? bucket_of(id, offset, E) : 0;
+        x.same = same_bucket(x.bucket, bits, live);
+        if (live && lane == __ffsll(x.same) - 1) atomicAdd(&mine[x.bucket], __popcll(x.same));
+        return x;
+    };
+    int id[BATCHES];
+#pragma unroll
+    for (int i = 0; i < BATCHES; ++i) id[i] = a + i * 64 + lane < z ? ids[a + i * 64 + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < BATCHES; ++i)
+        if (a + i * 64 < z) kept[i] = add(a + i * 64, id[i]);
+    for (int64_t s = a + BATCHES * 64; s < z; s += 64) add(s, s + lane < z ? ids[s + lane] : 0);
+}
+
+// Gives the slots their rows: mine[b] is the next row of bucket b.
+__device__ __forceinline__ void place_slots(const int32_t* ids, int64_t a, int64_t z, int k, int E,
+                                            long long offset, int bits, int* mine, const Batch (&kept)[BATCHES],
+                                            int32_t* token_of_row, int32_t* row_of_slot) {
+    const int lane = threadIdx.x & 63;
+    auto put = [&](int64_t s, const Batch& x) {
         const bool live = s + lane < z;
-        const int b = live ? bucket_of(ids[s + lane], offset, E) : 0;
-        const unsigned long long m = same_bucket(b, bits, live);
-        const int lead = m ? __ffsll(m) - 1 : 0;
+        const int lead = x.same ? __ffsll(x.same) - 1 : 0;
         int at = 0;
-        if (live && lane == lead) at = atomicAdd(&mine[b], __popcll(m));
+        if (live && lane == lead) at = atomicAdd(&mine[x.bucket], __popcll(x.same));
         at = __shfl(at, lead);
         if (live) {
-            const int row = at + __popcll(m & ((1ull << lane) - 1));
+            const int row = at + __popcll(x.same & ((1ull << lane) - 1));
             row_of_slot[s + lane] = row;
             token_of_row[row] = (int32_t)((s + lane) / k);
         }
+    };
+#pragma unroll
+    for (int i = 0; i < BATCHES; ++i)
+        if (a + i * 64 < z) put(a + i * 64, kept[i]);
+    for (int64_t s = a + BATCHES * 64; s < z; s += 64) {
+        Batch x;
+        const bool live = s + lane < z;
+        x.bucket = live ? bucket_of(ids[s + lane], offset, E) : 0;
+        x.same = same_bucket(x.bucket, bits, live);
+        put(s, x);
     }
 }
 
-// One workgroup. LDS: base [E + 1], counts [waves][E + 1], 16 wave sums.
+// One workgroup. LDS: counts [waves][E + 1], 16 wave sums.
 __global__ __launch_bounds__(1024) void sort_small_kernel(const int32_t* __restrict__ ids, int n, int k,
                                                           int E, long long offset, int bits,
                                                           int32_t* __restrict__ offsets,
                                                           int32_t* __restrict__ token_of_row,
                                                           int32_t* __restrict__ row_of_slot) {
     extern __shared__ int smem[];
-    int* base = smem;
-    int* counts = base + (E + 1);
-    int* tmp = counts + (blockDim.x >> 6) * (E + 1);
-    for (int i = threadIdx.x; i <= E; i += blockDim.x) base[i] = 0;
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int* counts = smem;
+    int* tmp = counts + waves * (E + 1);
+    for (int i = threadIdx.x; i < waves * (E + 1); i += blockDim.x) counts[i] = 0;
     __syncthreads();
-    for (int s = threadIdx.x; s < n; s += blockDim.x) atomicAdd(&base[bucket_of(ids[s], offset, E)], 1);
+    const int64_t per = ((n + waves - 1) / waves + 63) / 64 * 64;
+    const int64_t a = wave * per, z = min(a + per, (int64_t)n);
+    Batch kept[BATCHES];
+    count_slots(ids, a, z, E, offset, bits, counts + wave * (E + 1), kept);
     __syncthreads();
     int before = 0;
-    for (int b0 = 0; b0 < E; b0 += blockDim.x) {
+    for (int b0 = 0; b0 <= E; b0 += blockDim.x) {
         const int b = b0 + threadIdx.x;
-        int total;
-        const int at = before + block_scan(b < E ? base[b] : 0, tmp, &total);
-        if (b < E) {
-            offsets[b] = at;
-            base[b] = at;
+        int mine = 0, total;
+        if (b <= E)
+            for (int w = 0; w < waves; ++w) mine += counts[w * (E + 1) + b];
+        int at = before + block_scan(mine, tmp, &total);
+        if (b <= E) {
+            offsets[b] = at;  // [E]: where the other shards' slots start
+            for (int w = 0; w < waves; ++w) {
+                const int c = counts[w * (E + 1) + b];
+                counts[w * (E + 1) + b] = at;
+                at += c;
+            }
         }
         before += total;
     }
-    if (threadIdx.x == 0) {
-        offsets[E] = before;
-        base[E] = before;
-    }
     __syncthreads();
-    place(ids, 0, n, k, E, offset, bits, counts, base, token_of_row, row_of_slot);
+    place_slots(ids, a, z, k, E, offset, bits, counts + wave * (E + 1), kept, token_of_row, row_of_slot);
 }
 
 __global__ __launch_bounds__(512) void sort_count_kernel(const int32_t* __restrict__ ids, int64_t n,
@@ -168,15 +186,23 @@ __global__ __launch_bounds__(512) void sort_place_kernel(const int32_t* __restri
                                                          int32_t* __restrict__ token_of_row,
                                                          int32_t* __restrict__ row_of_slot) {
     extern __shared__ int smem[];
-    int* base = smem;
-    int* counts = base + (E + 1);
-    int* tmp = counts + (blockDim.x >> 6) * (E + 1);
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int* counts = smem;
+    int* tmp = counts + waves * (E + 1);
+    for (int i = threadIdx.x; i < waves * (E + 1); i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    const int64_t first = blockIdx.x * len, last = min(first + len, n);
+    const int64_t per = ((last - first + waves - 1) / waves + 63) / 64 * 64;
+    const int64_t a = first + wave * per, z = min(a + per, last);
+    Batch kept[BATCHES];
+    count_slots(ids, a, z, E, offset, bits, counts + wave * (E + 1), kept);
+    __syncthreads();
     int before = 0;  // rows of the buckets below this step's
     for (int b0 = 0; b0 <= E; b0 += blockDim.x) {
         const int b = b0 + threadIdx.x;
         int prior = 0, all = 0;
         if (b <= E) {
-#pragma unroll 8
+#pragma unroll 16
             for (int c = 0; c < (int)gridDim.x; ++c) {
                 const int v = chunk_counts[(int64_t)c * (E + 1) + b];
                 if (c < (int)blockIdx.x) prior += v;
@@ -184,16 +210,20 @@ __global__ __launch_bounds__(512) void sort_place_kernel(const int32_t* __restri
             }
         }
         int total;
-        const int at = before + block_scan(all, tmp, &total);
+        int at = before + block_scan(all, tmp, &total);
         if (b <= E) {
-            base[b] = at + prior;
             if (blockIdx.x == 0) offsets[b] = at;
+            at += prior;
+            for (int w = 0; w < waves; ++w) {
+                const int c = counts[w * (E + 1) + b];
+                counts[w * (E + 1) + b] = at;
+                at += c;
+            }
         }
         before += total;
     }
     __syncthreads();
-    const int64_t a = blockIdx.x * len;
-    place(ids, a, min(a + len, n), k, E, offset, bits, counts, base, token_of_row, row_of_slot);
+    place_slots(ids, a, z, k, E, offset, bits, counts + wave * (E + 1), kept, token_of_row, row_of_slot);
 }
 
 hipError_t launch_sort(const int32_t* ids, int64_t T, int k, int E, int64_t offset, int32_t* offsets,
@@ -207,10 +237,10 @@ hipError_t launch_sort(const int32_t* ids, int64_t T, int k, int E, int64_t offs
         int waves = (int)((n + 63) / 64), scan = (E + 63) / 64;
         if (scan > 4) scan = 4;
         if (waves < scan) waves = scan;
-        const int most = (int)((65536 - 64) / sizeof(int)) / (E + 1) - 1;
+        const int most = (int)((65536 - 64) / sizeof(int)) / (E + 1);
         if (waves > most) waves = most;
         if (waves > 16) waves = 16;
-        const size_t lds = ((size_t)(waves + 1) * (E + 1) + 16) * sizeof(int);
+        const size_t lds = ((size_t)waves * (E + 1) + 16) * sizeof(int);
         hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(64 * waves), lds, s, ids, (int)n, k, E,
                            (long long)offset, bits, offsets, token_of_row, row_of_slot);
         return hipGetLastError();
@@ -218,7 +248,7 @@ hipError_t launch_sort(const int32_t* ids, int64_t T, int k, int E, int64_t offs
     const int64_t len = chunk_len(n);
     hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)chunks), dim3(512), (E + 1) * sizeof(int), s, ids,
                        n, len, E, (long long)offset, counts);
-    const size_t lds = ((size_t)9 * (E + 1) + 16) * sizeof(int);
+    const size_t lds = ((size_t)8 * (E + 1) + 16) * sizeof(int);
     hipLaunchKernelGGL(sort_place_kernel, dim3((unsigned)chunks), dim3(512), lds, s, ids, n, len, k, E,
                        (long long)offset, bits, counts, offsets, token_of_row, row_of_slot);
     return hipGetLastError();
