@@ -31,6 +31,12 @@ __device__ __forceinline__ float element(const typename Vec<T, N>::type& v, int 
     else return (float)v[i];
 }
 
+// N elements that are read once: the load leaves nothing in the caches.
+template <class T, int N>
+__device__ __forceinline__ typename Vec<T, N>::type load_once(const T* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const typename Vec<T, N>::type*>(p));
+}
+
 template <class T, int N>
 __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
     if constexpr (N == 1) {
@@ -42,16 +48,26 @@ __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
     }
 }
 
-template <class T, int N>
+// STREAM: the store passes the caches by. (A run-time choice would not do: the
+// compiler makes one plain store of two that differ in this alone.)
+template <bool STREAM, class V>
+__device__ __forceinline__ void put(V* p, V v) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(v, p);
+    else
+        *p = v;
+}
+
+template <class T, int N, bool STREAM = false>
 __device__ __forceinline__ void store(T* p, const float (&v)[N]) {
+    typename Vec<T, N>::type w;
     if constexpr (N == 1) {
-        *p = (T)v[0];
+        w = (T)v[0];
     } else {
-        typename Vec<T, N>::type w;
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = (T)v[i];
-        *reinterpret_cast<typename Vec<T, N>::type*>(p) = w;
     }
+    put<STREAM>(reinterpret_cast<typename Vec<T, N>::type*>(p), w);
 }
 
 template <int N> struct IntC { static constexpr int value = N; };

@@ -36,6 +36,11 @@ inline unsigned blocks_for(int64_t T, int tx_log) {
     return (unsigned)(b < MAX_BLOCKS ? b : MAX_BLOCKS);
 }
 
+// Rows that all together exceed the 256 MB of the last cache are stored past
+// it: they would be gone before their reader comes, and what they push out has
+// to be written back meanwhile.
+inline bool streams(int64_t bytes) { return bytes > (int64_t)256 << 20; }
+
 // Rows of slots j0 .. j0 + KG - 1 of token t (-1 past the k of it), all loaded
 // before the first is used: loads and stores of rows in between would be
 // waited for with them, memory operations completing in order.
@@ -48,7 +53,7 @@ __device__ __forceinline__ void rows_of(const int32_t* row_of_slot, int64_t t, i
 }
 
 // V: the unit that moves, as wide as row length, strides and addresses allow.
-template <class V, bool ONE>
+template <class V, bool ONE, bool STREAM>
 __global__ __launch_bounds__(THREADS) void permute_kernel(const char* __restrict__ x, int64_t x_stride,
                                                           int64_t T, int k, int64_t vectors,
                                                           const int32_t* __restrict__ row_of_slot,
@@ -69,9 +74,9 @@ __global__ __launch_bounds__(THREADS) void permute_kernel(const char* __restrict
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
                 if (row[j] >= 0 && row[j] < local)
-                    reinterpret_cast<V*>(rows + row[j] * rows_stride)[v] = val;
+                    put<STREAM>(&reinterpret_cast<V*>(rows + row[j] * rows_stride)[v], val);
                 else if (zero_rest && row[j] >= 0 && row[j] < R)
-                    reinterpret_cast<V*>(rows + row[j] * rows_stride)[v] = V{};
+                    put<STREAM>(&reinterpret_cast<V*>(rows + row[j] * rows_stride)[v], V{});
             }
         }
     }
@@ -87,7 +92,9 @@ hipError_t launch_permute(const void* x, int64_t x_stride, int64_t T, int k, int
         const int64_t vectors = row_bytes / (int64_t)sizeof(V);
         const int tx_log = lanes_log(vectors);
         const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
-        const auto kernel = tx_log >= 6 ? permute_kernel<V, true> : permute_kernel<V, false>;
+        const bool stream = streams(T * k * row_bytes);
+        const auto kernel = tx_log >= 6 ? (stream ? permute_kernel<V, true, true> : permute_kernel<V, true, false>)
+                                        : (stream ? permute_kernel<V, false, true> : permute_kernel<V, false, false>);
         hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, s, (const char*)x, x_stride, T, k, vectors, row_of_slot,
                            num_rows, (char*)rows, rows_stride, (int)zero_rest, tx_log);
         return hipGetLastError();
@@ -129,7 +136,7 @@ __global__ __launch_bounds__(THREADS) void unpermute_kernel(const T* __restrict_
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
                 on[j] = row[j] >= 0 && row[j] < local;
-                if (on[j]) v[j] = *reinterpret_cast<const typename Vec<T, N>::type*>(rows + row[j] * rows_stride + c);
+                if (on[j]) v[j] = load_once<T, N>(rows + row[j] * rows_stride + c);
             }
 #pragma unroll
             for (int j = 0; j < KG; ++j)
@@ -147,7 +154,7 @@ __global__ __launch_bounds__(THREADS) void unpermute_kernel(const T* __restrict_
 
 // Gradients of a token's rows and weights: its tx lanes walk the columns, each
 // lane keeps one partial product sum per slot, and the sums meet at the end.
-template <class T, int N, bool ONE>
+template <class T, int N, bool ONE, bool STREAM>
 __global__ __launch_bounds__(THREADS) void unpermute_backward_kernel(
     const T* __restrict__ grad, int64_t grad_stride, const T* __restrict__ rows, int64_t rows_stride,
     int64_t tokens, int k, int64_t H, const int32_t* __restrict__ row_of_slot,
@@ -176,27 +183,25 @@ __global__ __launch_bounds__(THREADS) void unpermute_backward_kernel(
                 for (int64_t c = (int64_t)lane * N; c < H; c += (int64_t)tx * N) {
                     float g[N];
                     load<T, N>(grad + t * grad_stride + c, g);
+                    typename Vec<T, N>::type v[KG];
+                    if (grad_weights) {
+#pragma unroll
+                        for (int j = 0; j < KG; ++j)
+                            if (row[j] >= 0 && row[j] < local) v[j] = load_once<T, N>(rows + row[j] * rows_stride + c);
+                    }
 #pragma unroll
                     for (int j = 0; j < KG; ++j) {
-                        if (row[j] < 0) continue;
-                        if (row[j] < local) {
-                            if (grad_weights) {
-                                float v[N];
-                                load<T, N>(rows + row[j] * rows_stride + c, v);
+                        const bool on = row[j] >= 0 && row[j] < local;
+                        if (row[j] < 0 || !(on || zero_rest)) continue;
+                        if (on && grad_weights) {
 #pragma unroll
-                                for (int i = 0; i < N; ++i) dot[j] = fmaf(g[i], v[i], dot[j]);
-                            }
-                            if (grad_rows) {
-                                float d[N];
-#pragma unroll
-                                for (int i = 0; i < N; ++i) d[i] = w[j] * g[i];
-                                store<T, N>(grad_rows + row[j] * grad_rows_stride + c, d);
-                            }
-                        } else if (grad_rows && zero_rest) {
+                            for (int i = 0; i < N; ++i) dot[j] = fmaf(g[i], element<T, N>(v[j], i), dot[j]);
+                        }
+                        if (grad_rows) {
                             float d[N];
 #pragma unroll
-                            for (int i = 0; i < N; ++i) d[i] = 0.f;
-                            store<T, N>(grad_rows + row[j] * grad_rows_stride + c, d);
+                            for (int i = 0; i < N; ++i) d[i] = on ? w[j] * g[i] : 0.f;
+                            store<T, N, STREAM>(grad_rows + row[j] * grad_rows_stride + c, d);
                         }
                     }
                 }
@@ -267,7 +272,11 @@ hipError_t launch_unpermute_backward(int dtype, const void* grad, int64_t grad_s
         typedef decltype(elem) E;
         constexpr int N = decltype(width)::value;
         const int tx_log = lanes_log((H + N - 1) / N);
-        const auto kernel = tx_log >= 6 ? unpermute_backward_kernel<E, N, true> : unpermute_backward_kernel<E, N, false>;
+        const bool stream = streams(T * k * H * (int64_t)sizeof(E));
+        const auto kernel =
+            tx_log >= 6
+                ? (stream ? unpermute_backward_kernel<E, N, true, true> : unpermute_backward_kernel<E, N, true, false>)
+                : (stream ? unpermute_backward_kernel<E, N, false, true> : unpermute_backward_kernel<E, N, false, false>);
         hipLaunchKernelGGL(kernel, dim3(blocks_for(T, tx_log)), dim3(THREADS), 0, s, (const E*)grad, grad_stride,
                            (const E*)rows, rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)grad_rows,
                            grad_rows_stride, (int)zero_rest, grad_weights, tx_log);
