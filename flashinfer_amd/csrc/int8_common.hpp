@@ -22,6 +22,7 @@ struct Int8Call {
     int64_t a_stride, b_stride, b_expert_stride, out_stride;
     int E;
     int bias_dtype;
+    int b_large;  // the weights exceed the 256 MB of the last cache
 };
 
 // v_mfma_i32_16x16x64_i8: lane l gives 16 bytes of row l % 16 of each operand

@@ -17,21 +17,22 @@ bool int8_offsets_fit(const Int8Call& p, int bm, int bn) {
 
 // The tile of a product. Tiles are taken as large as still give each CU one
 // (256 of them), and K is shared inside a workgroup where that is what is left
-// to share. wide: 256 x 256 tiles are there too (Int8Tile::T256x256).
+// to share. Experts with more tiles than that take tiles that hold their rows,
+// so that their weights are read once: those are what bounds the call. (Rows
+// of an expert: as many as there are at most, on average.) wide: 256 x 256
+// tiles are there too.
 Int8Tile pick_tile(const Int8Call& p, bool wide) {
-    auto tiles = [&](int bm, int bn) { return (p.rows + bm - 1) / bm * ((p.N + bn - 1) / bn); };
-    if (p.offsets) {
-        const int64_t rows = p.rows / p.E;  // of an expert, on average and at most
-        if (rows <= 40) return Int8Tile::T64x128;
-        return rows <= 96 || !wide ? Int8Tile::T128x128 : Int8Tile::T256x256;
-    }
+    const int64_t groups = p.offsets ? p.E : 1, rows = (p.rows + groups - 1) / groups;
+    auto tiles = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
     if (tiles(32, 32) <= 256) return Int8Tile::T32x32;
     if (tiles(32, 64) <= 256) return Int8Tile::T32x64;
     if (tiles(64, 64) <= 256) return Int8Tile::T64x64_K2;
     if (tiles(64, 64) <= 512 && p.K <= 2048) return Int8Tile::T64x64;
     if (tiles(64, 128) <= 256) return Int8Tile::T64x128_K2;
+    if (p.offsets && rows <= 40) return Int8Tile::T64x128;
     if (tiles(128, 128) <= 256) return Int8Tile::T128x128_K2;
-    return tiles(128, 128) <= 512 || !wide ? Int8Tile::T128x128 : Int8Tile::T256x256;
+    if (tiles(128, 128) <= 512 || !wide || (p.offsets && rows <= 96)) return Int8Tile::T128x128;
+    return Int8Tile::T256x256;
 }
 
 // MI_INT8_TILE = 0 .. 8 (an Int8Tile) takes that tile where a call can have it, for tests and timing.
@@ -64,6 +65,7 @@ hipError_t launch_int8_matmul(const mi_experts_int8_args& a, hipStream_t s) {
     p.out_stride = a.out_stride;
     p.E = a.num_experts;
     p.bias_dtype = a.bias_dtype;
+    p.b_large = (a.num_experts ? a.num_experts : 1) * a.N * a.K > ((int64_t)256 << 20);
     const uint64_t bits = (uint64_t)p.a | (uint64_t)p.b | (uint64_t)p.a_stride | (uint64_t)p.b_stride |
                           (uint64_t)p.b_expert_stride;
     const uint64_t quad = a.out_dtype == MI_EXPERTS_F32 ? 16 : 8;

@@ -15,8 +15,8 @@
 
 namespace miexp {
 
-using mimoe::g2l16;
 using mimoe::g2l16s;
+using mimoe::g2l16s_once;
 using mimoe::swzq;
 
 template <int N>
@@ -24,17 +24,13 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <class T, int BM, int BN, int STAGES, int KS>
-__global__ __launch_bounds__(256 * KS) void int8_tile_kernel(Int8Call p, int ntiles, int vec) {
+// ONCE: the weights pass the caches by.
+template <class T, int BM, int BN, int STAGES, int KS, bool ONCE>
+__device__ __forceinline__ void tile_run(const Int8Call& p, uint8_t* smem, int e, int64_t row0, int nrows, int n0,
+                                         bool vec) {
     constexpr int MT = BM / 32, NT = BN / 32;  // 16 x 16 tiles of a wave
     constexpr int A_LD = BM / 32, B_LD = BN / 32, LD = A_LD + B_LD;  // 1 KB copies of a wave
     constexpr int STAGE = (BM + BN) * 128;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[KS * STAGES * STAGE];
-    static_assert(sizeof(smem) <= 160 * 1024 && (KS - 1) * BM * BN * 4 <= (int)sizeof(smem), "LDS budget");
-    int e, nrows;
-    int64_t row0;
-    if (!find_tile<BM>(p, blockIdx.x / ntiles, e, row0, nrows)) return;
-    const int n0 = (int)(blockIdx.x % ntiles) * BN;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
     const int ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
@@ -78,8 +74,12 @@ __global__ __launch_bounds__(256 * KS) void int8_tile_kernel(Int8Call p, int nti
         const uint32_t last = kb == KB - 1 ? ~0u : 0u;
 #pragma unroll
         for (int i = 0; i < LD; ++i)
-            g2l16s(i < A_LD ? a : b, off[i] - (cut[i] & last),
-                   s + (i < A_LD ? wave * A_LD + i : BM / 8 + wave * B_LD + i - A_LD) * 1024);
+            if (i < A_LD)
+                g2l16s(a, off[i] - (cut[i] & last), s + (wave * A_LD + i) * 1024);
+            else if (ONCE)
+                g2l16s_once(b, off[i] - (cut[i] & last), s + (BM / 8 + wave * B_LD + i - A_LD) * 1024);
+            else
+                g2l16s(b, off[i] - (cut[i] & last), s + (BM / 8 + wave * B_LD + i - A_LD) * 1024);
     };
     v4i acc[MT][NT];
 #pragma unroll
@@ -132,6 +132,24 @@ __global__ __launch_bounds__(256 * KS) void int8_tile_kernel(Int8Call p, int nti
     if (ks > 0) return;
     store_tiles<T, MT, NT>(p, e, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec,
                            [&](int m, int n) { return acc[m][n]; });
+}
+
+template <class T, int BM, int BN, int STAGES, int KS>
+__global__ __launch_bounds__(256 * KS) void int8_tile_kernel(Int8Call p, int ntiles, int vec) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[KS * STAGES * (BM + BN) * 128];
+    static_assert(sizeof(smem) <= 160 * 1024 && (KS - 1) * BM * BN * 4 <= (int)sizeof(smem), "LDS budget");
+    Tiles x;
+    const int mt = blockIdx.x / ntiles, n0 = (int)(blockIdx.x % ntiles) * BN;
+    if (!find_expert<BM>(p, mt, x)) return;
+    const int64_t row0 = (int64_t)x.row + (int64_t)(mt - x.first) * BM;
+    const int nrows = (int)min((int64_t)BM, x.end - row0);
+    // Weights that no other row tile reads, of more than the last cache holds
+    // (32 experts of 4096 x 7168, 64 rows each: 177 -> 164 us; with two row
+    // tiles or more, or weights that stay cached from call to call, it costs).
+    if (x.tiles == 1 && p.b_large)
+        tile_run<T, BM, BN, STAGES, KS, true>(p, smem, x.e, row0, nrows, n0, vec);
+    else
+        tile_run<T, BM, BN, STAGES, KS, false>(p, smem, x.e, row0, nrows, n0, vec);
 }
 
 template <int BM, int BN, int STAGES, int KS>

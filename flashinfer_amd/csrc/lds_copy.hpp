@@ -47,6 +47,14 @@ __device__ __forceinline__ void g2l16s(const void* sbase, uint32_t voff, void* l
                  : "memory", "m0");
 }
 
+// g2l16s for data that nothing reads again: it leaves nothing in the caches.
+__device__ __forceinline__ void g2l16s_once(const void* sbase, uint32_t voff, void* lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(voff), "s"(sbase), "s"(lds_addr(lds_base))
+                 : "memory", "m0");
+}
+
 __device__ __forceinline__ void g2l4s(const void* sbase, uint32_t voff, void* lds_base) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                  :
