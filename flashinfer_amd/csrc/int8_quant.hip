@@ -8,9 +8,9 @@
 // gets a scale that is not finite, and zeros, so that its products are NaN
 // instead of numbers made without it.
 //
-// A wave (rows up to 1024 elements) or a workgroup takes a row. Its first
-// CACHED vectors per lane stay in registers between the two passes; longer
-// rows are read (and, with SwiGLU, computed) again from L2. Bound by HBM.
+// TX lanes (a wave or a workgroup) take a row. Its first CACHED vectors per
+// lane stay in registers between the two passes; longer rows are read (and,
+// with SwiGLU, computed) again. Bound by HBM.
 #include "experts_common.hpp"
 
 namespace miexp {
@@ -18,14 +18,40 @@ namespace miexp {
 constexpr float INT8_MAX_F = 127.f;
 constexpr float QUANT_FLOOR = 1e-10f;  // scale of an all-zero row: that of quantize_activations
 
+// v = g * u / (1 + exp(-u)). The exponential is 2^(hi + lo) with hi + lo =
+// -u log2(e) to twice the precision, the quotient a reciprocal and one Newton
+// step: within 6 * 2^-24 of the value, in half the instructions of a library
+// exponential and an IEEE division, which bound this kernel. Where 1 + exp(-u)
+// leaves the reciprocal's range, those are what is computed.
+template <int N>
+__device__ __forceinline__ void swiglu(float (&v)[N], const float (&u)[N]) {
+    constexpr float L2E = 1.44269502f, L2E_LO = 1.92596299e-8f, LN2 = 0.693147182f;
+    float s[N];
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float hi = -u[i] * L2E, lo = fmaf(-u[i], L2E_LO, fmaf(-u[i], L2E, -hi));
+        float x = __builtin_amdgcn_exp2f(hi);
+        x = fmaf(x, lo * LN2, x);
+        far |= !(u[i] > -87.f);
+        const float d = 1.f + x, rc = __builtin_amdgcn_rcpf(d), q = u[i] * rc;
+        s[i] = fmaf(fmaf(-q, d, u[i]), rc, q);
+    }
+    if (far) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = u[i] / (1.f + expf(-u[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= s[i];
+}
+
 template <class T, int N, bool SWIGLU>
 __device__ __forceinline__ void quant_input(const T* row, int64_t K, int64_t c, float (&v)[N]) {
     load<T, N>(row + c, v);
     if constexpr (SWIGLU) {
         float u[N];
         load<T, N>(row + K + c, u);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= u[i] / (1.f + expf(-u[i]));
+        swiglu(v, u);
     }
 }
 
@@ -49,14 +75,29 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
             for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(w[i]) & 0x7fffffffu);
         };
         if (live) {
+            // all loads before the first use
+            typename Vec<T, N>::type g[CACHED], u[CACHED];
 #pragma unroll
             for (int i = 0; i < CACHED; ++i) {
                 const int64_t c = ((int64_t)i * TX + lane) * N;
-                if (c < K) quant_input<T, N, SWIGLU>(row, K, c, v[i]);
+                if (c < K) {
+                    g[i] = *reinterpret_cast<const typename Vec<T, N>::type*>(row + c);
+                    if (SWIGLU) u[i] = *reinterpret_cast<const typename Vec<T, N>::type*>(row + K + c);
+                }
             }
 #pragma unroll
-            for (int i = 0; i < CACHED; ++i)
-                if (((int64_t)i * TX + lane) * N < K) take(v[i]);
+            for (int i = 0; i < CACHED; ++i) {
+                if (((int64_t)i * TX + lane) * N >= K) continue;
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i][e] = element<T, N>(g[i], e);
+                if constexpr (SWIGLU) {
+                    float w[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) w[e] = element<T, N>(u[i], e);
+                    swiglu(v[i], w);
+                }
+                take(v[i]);
+            }
             for (int64_t c = ((int64_t)CACHED * TX + lane) * N; c < K; c += (int64_t)TX * N) {
                 float w[N];
                 quant_input<T, N, SWIGLU>(row, K, c, w);
@@ -75,10 +116,32 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
         const bool finite = top < 0x7f800000u;
         const float amax = __uint_as_float(top);
         const float s = finite ? fmaxf(amax, QUANT_FLOOR) / INT8_MAX_F : amax;
+        const float inverse = 1.f / s;  // finite: s >= 7.8e-13
         auto put = [&](int64_t c, const float (&w)[N]) {
             int8_t b[N];
+            if constexpr (SWIGLU) {
+                // rint(w / s) by a product with 1 / s, whose error is below
+                // 127 * 2^-22 = 3.1e-5, unless that could change a rounding.
+                // (The plain quantiser has the time for its divisions: 41
+                // against 49 us at 8192 x 7168; here it is 80 against 63.)
+                float x[N];
+                bool tie = false;
 #pragma unroll
-            for (int i = 0; i < N; ++i) b[i] = finite ? (int8_t)(int)rintf(w[i] / s) : (int8_t)0;
+                for (int i = 0; i < N; ++i) {
+                    const float y = w[i] * inverse;
+                    x[i] = rintf(y);
+                    tie |= !(fabsf(y - x[i]) < 0.4999f);
+                }
+                if (tie) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) x[i] = finite ? rintf(w[i] / s) : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) b[i] = (int8_t)(int)x[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) b[i] = finite ? (int8_t)(int)rintf(w[i] / s) : (int8_t)0;
+            }
             if constexpr (N == 8)
                 *reinterpret_cast<uint2*>(q + m * q_stride + c) = *reinterpret_cast<const uint2*>(b);
             else if constexpr (N == 4)
@@ -115,8 +178,13 @@ hipError_t launch_quantize(int dtype, const void* x, int64_t x_stride, int64_t M
                                (const E*)x, x_stride, M, K, num_rows, q, q_stride, scale);
             return hipGetLastError();
         };
-        if (K <= 1024)
+        // A wave for a short row, and where there are rows enough to fill the
+        // chip with waves; a workgroup for a row else (8192 x 2048: 14.7 against
+        // 16.9 us; 4096 x 4096: 16.7 against 14.2).
+        if (K <= 128 * N && (K <= 64 * N || M >= 512))
             return swiglu ? launch(quantize_kernel<E, N, true, 2, 64>, 4) : launch(quantize_kernel<E, N, false, 2, 64>, 4);
+        if (K <= 256 * N && M >= 2048)
+            return swiglu ? launch(quantize_kernel<E, N, true, 4, 64>, 4) : launch(quantize_kernel<E, N, false, 4, 64>, 4);
         return swiglu ? launch(quantize_kernel<E, N, true, 4, 256>, 1) : launch(quantize_kernel<E, N, false, 4, 256>, 1);
     };
     const uint64_t size = dtype == MI_EXPERTS_F32 ? 4 : 2;
