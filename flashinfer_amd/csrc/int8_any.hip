@@ -80,6 +80,8 @@ __global__ __launch_bounds__(256 * KS) void int8_any_kernel(Int8Call p, int ntil
             *reinterpret_cast<v4i*>(mine + stage * STAGE + row * 128 + ((chunk ^ swzq(row)) << 4)) = held[i];
         }
     };
+    Scales<MT, NT> scales;
+    scales.load(p, e, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2));
     v4i acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -114,8 +116,7 @@ __global__ __launch_bounds__(256 * KS) void int8_any_kernel(Int8Call p, int ntil
     }
     sum_groups<KS, MT, NT>(smem, ks, wave, acc);
     if (ks > 0) return;
-    store_tiles<T, MT, NT>(p, e, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec,
-                           [&](int m, int n) { return acc[m][n]; });
+    store_tiles<T>(p, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec, acc, scales);
 }
 
 template <int BM, int BN, int KS>

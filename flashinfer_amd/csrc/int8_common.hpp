@@ -152,60 +152,64 @@ __device__ __forceinline__ float row_scale(const Int8Call& p, int64_t row) {
     return from >= 0 ? p.a_scale[from] : __builtin_nanf("");
 }
 
-// Scales and bias of four neighbouring channels n .. n + 3 of expert e.
-struct Channels {
-    float s[4], b[4];
-    __device__ __forceinline__ Channels(const Int8Call& p, int e, int n) {
+// The scales and biases of a wave's MT x NT tiles: rows row_at + 16 m +
+// lane % 16 of the tile, channels n_at + 16 n + 4 (lane / 16) .. Loaded before
+// the products, used after them.
+template <int MT, int NT>
+struct Scales {
+    float a[MT];
+    float s[NT][4], b[NT][4];
+
+    __device__ __forceinline__ void load(const Int8Call& p, int e, int64_t row0, int nrows, int row_at, int n_at) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int row = row_at + m * 16 + (lane & 15);
+            a[m] = row < nrows ? row_scale(p, row0 + row) : 0.f;
+        }
         const float* scale = p.b_scale + (int64_t)e * p.N;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s[v] = scale[min(n + v, p.N - 1)];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) b[v] = 0.f;
+            for (int v = 0; v < 4; ++v) {
+                s[n][v] = scale[min(n_at + n * 16 + 4 * (lane >> 4) + v, p.N - 1)];
+                b[n][v] = 0.f;
+            }
         if (p.bias) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) b[v] = bias_at(p, min(n + v, p.N - 1));
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) b[n][v] = bias_at(p, min(n_at + n * 16 + 4 * (lane >> 4) + v, p.N - 1));
         }
     }
 };
 
-// The four outputs of a row at out (channels n ..) from their integer sums.
-// vec: rows of out hold aligned groups of four.
-template <class T>
-__device__ __forceinline__ void finish4(T* out, int n, int N, const v4i& acc, float sa, const Channels& c, bool vec) {
-    float y[4];
-#pragma unroll
-    for (int v = 0; v < 4; ++v) y[v] = (float)acc[v] * sa * c.s[v] + c.b[v];
-    if (vec && n + 4 <= N) {
-        store<T, 4>(out, y);
-        return;
-    }
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-        if (n + v < N) out[v] = (T)y[v];
-}
-
-// A wave's MT x NT sums: rows row_at + 16 m + lane % 16 of the tile, channels
-// n_at + 16 n + 4 (lane / 16) ... ACC(m, n) gives the sums.
-template <class T, int MT, int NT, class ACC>
-__device__ __forceinline__ void store_tiles(const Int8Call& p, int e, int64_t row0, int nrows, int row_at, int n_at,
-                                            bool vec, ACC acc) {
+// Stores a wave's tiles from their sums. vec: rows of out hold aligned groups
+// of four.
+template <class T, int MT, int NT>
+__device__ __forceinline__ void store_tiles(const Int8Call& p, int64_t row0, int nrows, int row_at, int n_at, bool vec,
+                                            const v4i (&acc)[MT][NT], const Scales<MT, NT>& c) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    float sa[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = row_at + m * 16 + r;
-        sa[m] = row < nrows ? row_scale(p, row0 + row) : 0.f;
-    }
     T* out = reinterpret_cast<T*>(p.out) + (row0 + row_at + r) * p.out_stride;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int at = n_at + n * 16 + 4 * g;
         if (at >= p.N) break;
-        const Channels c(p, e, at);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-            if (row_at + m * 16 + r < nrows)
-                finish4<T>(out + m * 16 * p.out_stride + at, at, p.N, acc(m, n), sa[m], c, vec);
+        for (int m = 0; m < MT; ++m) {
+            if (row_at + m * 16 + r >= nrows) continue;
+            T* to = out + m * 16 * p.out_stride + at;
+            float y[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) y[v] = (float)acc[m][n][v] * c.a[m] * c.s[n][v] + c.b[n][v];
+            if (vec && at + 4 <= p.N) {
+                store<T, 4>(to, y);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (at + v < p.N) to[v] = (T)y[v];
+            }
+        }
     }
 }
 

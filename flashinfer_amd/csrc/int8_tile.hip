@@ -81,6 +81,8 @@ __device__ __forceinline__ void tile_run(const Int8Call& p, uint8_t* smem, int e
             else
                 g2l16s(b, off[i] - (cut[i] & last), s + (BM / 8 + wave * B_LD + i - A_LD) * 1024);
     };
+    Scales<MT, NT> scales;
+    scales.load(p, e, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2));
     v4i acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -130,8 +132,7 @@ __device__ __forceinline__ void tile_run(const Int8Call& p, uint8_t* smem, int e
     turn(turns - 1, IntC<1>{});
     sum_groups<KS, MT, NT>(smem, ks, wave, acc);
     if (ks > 0) return;
-    store_tiles<T, MT, NT>(p, e, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec,
-                           [&](int m, int n) { return acc[m][n]; });
+    store_tiles<T>(p, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec, acc, scales);
 }
 
 template <class T, int BM, int BN, int STAGES, int KS>
