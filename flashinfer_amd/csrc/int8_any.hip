@@ -29,6 +29,23 @@ __device__ __forceinline__ v4i row16(const int8_t* p, int k, int K) {
     return __builtin_bit_cast(v4i, x);
 }
 
+// Rows of K bytes at any address -> rows of ld bytes (a multiple of 16), zeros
+// past K: the rows of a, then those of b.
+__global__ __launch_bounds__(256) void pack_rows_kernel(Int8Call p, int8_t* __restrict__ to, int ld) {
+    for (int64_t row = blockIdx.x; row < p.a_rows + p.N; row += gridDim.x) {
+        const int8_t* from = row < p.a_rows ? p.a + row * p.a_stride : p.b + (row - p.a_rows) * p.b_stride;
+        for (int k = threadIdx.x * 16; k < ld; k += 256 * 16)
+            *reinterpret_cast<v4i*>(to + row * ld + k) = row16(from, k, p.K);
+    }
+}
+
+hipError_t launch_pack_rows(const Int8Call& p, int8_t* to, int ld, hipStream_t s) {
+    const int64_t rows = p.a_rows + p.N;
+    hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(rows < MAX_BLOCKS ? rows : MAX_BLOCKS)), dim3(256), 0, s, p,
+                       to, ld);
+    return hipGetLastError();
+}
+
 template <class T, int BM, int BN, int KS>
 __global__ __launch_bounds__(256 * KS) void int8_any_kernel(Int8Call p, int ntiles, int vec) {
     constexpr int MT = BM / 32, NT = BN / 32;        // 16 x 16 tiles of a wave

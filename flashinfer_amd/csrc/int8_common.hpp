@@ -243,6 +243,7 @@ inline int64_t max_tiles(int64_t rows, int bm, int E) {
 // multiples of 16.
 bool int8_offsets_fit(const Int8Call& p, int bm, int bn);  // a tile's lane offsets within 32 bits
 enum class Int8Tile { T32x32, T32x64, T64x64_K2, T64x64, T64x128_K2, T64x128, T128x128_K2, T128x128, T256x256 };
+hipError_t launch_pack_rows(const Int8Call& p, int8_t* to, int ld, hipStream_t s);
 hipError_t launch_int8_any(const Int8Call& p, int out_dtype, Int8Tile tile, bool vec, hipStream_t s);
 hipError_t launch_int8_tile(const Int8Call& p, int out_dtype, Int8Tile tile, bool vec, hipStream_t s);
 hipError_t launch_int8_wide(const Int8Call& p, int out_dtype, hipStream_t s);

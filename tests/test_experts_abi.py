@@ -123,6 +123,15 @@ def test_int8_matmul_refuses():
         a = Args(**dict(base, **change))
         rc, msg = call("mi_experts_int8_matmul", [ctypes.POINTER(Args), ptr], [ctypes.byref(a), None])
         assert rc == 1 and word in msg, (change, rc, msg)
+    # rows of no multiple of 16 bytes are copied from a size on
+    copied = dict(good, a_rows=4096, rows=4096, N=4096, K=1025, a_stride=1025, b_stride=1025, out_stride=4096)
+    need = lib().mi_experts_int8_workspace_size(i64(4096), i64(4096), i64(1025), i32(0))
+    assert need == 8192 * 1040
+    for workspace, nbytes, code, word in ((None, 0, 2, "workspace"), (P, need - 1, 2, "workspace"), (P + 16, need, 1, "misaligned")):
+        a = Args(**dict(copied, workspace=workspace, workspace_bytes=nbytes))
+        rc, msg = call("mi_experts_int8_matmul", [ctypes.POINTER(Args), ptr], [ctypes.byref(a), None])
+        assert rc == code and word in msg, (workspace, rc, msg)
+    assert lib().mi_experts_int8_workspace_size(i64(4096), i64(4096), i64(1024), i32(0)) == 0
     rc, msg = call("mi_experts_int8_matmul", [ctypes.POINTER(Args), ptr], [None, None])
     assert rc == 1 and "NULL" in msg
 

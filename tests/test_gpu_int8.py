@@ -49,7 +49,8 @@ SHAPES = [  # M, N, K
     (1, 1, 1), (1, 16, 64), (1, 4096, 7168), (2, 100, 4096), (3, 17, 33), (5, 64, 128), (16, 4096, 2048),
     (17, 130, 1024), (31, 48, 272), (33, 1000, 528), (64, 256, 7168), (65, 64, 16), (100, 7168, 2048),
     (128, 128, 128), (130, 515, 1040), (200, 4096, 512), (256, 256, 256), (257, 300, 130), (300, 264, 784),
-    (511, 513, 96), (600, 1024, 2048), (1024, 2048, 1024), (1111, 999, 400), (2050, 1536, 4096), (4097, 31, 160)]
+    (511, 513, 96), (600, 1024, 2048), (1024, 2048, 1024), (1111, 999, 400), (2050, 1536, 4096), (4097, 31, 160),
+    (2049, 2050, 4101), (8200, 4100, 1025)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
