@@ -94,6 +94,38 @@ void expect_out(const Tensor& t, const char* name, at::ScalarType type, at::IntA
     TORCH_CHECK_VALUE(t.dim() != 1 || t.is_contiguous(), name, " must be contiguous");
 }
 
+// Bytes a tensor's elements lie in.
+std::pair<const char*, const char*> extent(const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const char* p = static_cast<const char*>(t.const_data_ptr());
+    return {p, p + (last + 1) * (int64_t)t.element_size()};
+}
+
+// A destination shares no memory with what is read: rows are written while
+// others are read. Columns of one buffer may be both.
+void expect_apart(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+    if (out.numel() == 0) return;
+    const auto o = extent(out);
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || t->numel() == 0) continue;
+        const auto i = extent(*t);
+        if (i.second <= o.first || o.second <= i.first) continue;
+        if (t->dim() == 2 && out.dim() == 2 && t->size(0) > 1 && out.size(0) > 1) {
+            const int64_t pitch = out.stride(0) * (int64_t)out.element_size();
+            if (pitch > 0 && t->stride(0) * (int64_t)t->element_size() == pitch && t->stride(1) == 1) {
+                const int64_t w = t->size(1) * (int64_t)t->element_size(), n = out.size(1) * (int64_t)out.element_size();
+                const int64_t at = ((i.first - o.first) % pitch + pitch) % pitch;
+                if (at >= n && at + w <= pitch) continue;
+            }
+        }
+        TORCH_CHECK_VALUE(false, name, " shares memory with a tensor that the call reads");
+    }
+}
+
+// Writes through a pointer are in-place changes to autograd, too.
+void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
 void no_grad_out(const char* what, bool needs, const OptTensor& out) {
     TORCH_CHECK_VALUE(!(out && out->defined() && (needs || (at::GradMode::is_enabled() && out->requires_grad()))),
                       what, "(): out= takes no part in autograd; call it without out, or under torch.no_grad()");
@@ -200,6 +232,8 @@ Tensor permute(const Tensor& hidden, const Tensor& offsets, const Tensor& row_of
     no_grad_out("permute", needs, out);
     if (out && out->defined()) {
         expect_out(*out, "out", hidden.scalar_type(), {p.T * p.k, hidden.size(1)}, hidden);
+        expect_apart(*out, "out", {&hidden, &p.row_of_slot, &p.offsets});
+        written(*out);
         permute_into(hidden, p, *out, false);
         return *out;
     }
@@ -266,6 +300,8 @@ Tensor unpermute(const Tensor& rows, const Tensor& offsets, const Tensor& row_of
     no_grad_out("unpermute", needs, out);
     if (out && out->defined()) {
         expect_out(*out, "out", rows.scalar_type(), {p.T, rows.size(1)}, rows);
+        expect_apart(*out, "out", {&rows, &w, &p.row_of_slot, &p.offsets});
+        written(*out);
         if (out->numel() == 0) return *out;
         On on(rows);
         const Tensor in = rows_of(rows), wc = w.defined() ? w.contiguous() : w;
@@ -306,8 +342,17 @@ py::tuple quantize(const Tensor& x, bool swiglu, const OptTensor& num_rows, cons
     expect_no_grad(swiglu ? "swiglu_quantize_int8" : "quantize_int8", {&x});
     On on(x);
     const bool given_q = q_out && q_out->defined(), given_s = scale_out && scale_out->defined();
-    if (given_q) expect_out(*q_out, "q", at::kChar, {M, K}, x);
-    if (given_s) expect_out(*scale_out, "scale", at::kFloat, {M}, x);
+    const Tensor none, &count = num_rows ? *num_rows : none;
+    if (given_q) {
+        expect_out(*q_out, "q", at::kChar, {M, K}, x);
+        expect_apart(*q_out, "q", {&x, &count});
+        written(*q_out);
+    }
+    if (given_s) {
+        expect_out(*scale_out, "scale", at::kFloat, {M}, x);
+        expect_apart(*scale_out, "scale", {&x, &count, given_q ? &*q_out : &none});
+        written(*scale_out);
+    }
     const auto opt = x.options().requires_grad(false);
     const bool cut = num_rows && num_rows->defined();
     auto fresh = [&](at::IntArrayRef shape, at::ScalarType t) {
@@ -378,7 +423,14 @@ Tensor int8_call(const Tensor& a, const Tensor& a_scale, const Tensor& b, const 
     if (given) expect_no_grad(grouped ? "int8_grouped_matmul" : "int8_matmul", {&*out_opt});
     if (given) out_type = out_opt->scalar_type();
     c.out_dtype = out_dtype_of(out_type);
-    if (given) expect_out(*out_opt, "out", out_type, {rows, N}, a);
+    TORCH_CHECK_VALUE(M > 0 || rows == 0, "a has no rows, row_ids ", rows);
+    if (given) {
+        const Tensor none;
+        expect_out(*out_opt, "out", out_type, {rows, N}, a);
+        expect_apart(*out_opt, "out", {&a, &a_scale, &b, &b_scale, bias ? &*bias : &none,
+                                       offsets ? offsets : &none, row_ids ? &*row_ids : &none});
+        written(*out_opt);
+    }
     On on(a);
     const auto opt = a.options().requires_grad(false).dtype(out_type);
     // rows that no expert has are not written by a grouped product

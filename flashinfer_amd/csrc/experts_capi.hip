@@ -206,9 +206,8 @@ int mi_experts_int8_matmul(const mi_experts_int8_args* args, void* stream) {
         return fail(MI_EXPERTS_ERR_INVALID, "%s: %lld x %lld outputs are too many for one call", who,
                     (long long)a.rows, (long long)a.N);
     if (a.rows == 0 || a.N == 0) return MI_EXPERTS_OK;
-    if ((!a.a || !a.a_scale) && a.a_rows > 0)
-        return fail(MI_EXPERTS_ERR_INVALID, "%s: NULL pointer argument", who);
-    if (!a.b || !a.b_scale || !a.out || (a.num_experts && !a.expert_offsets))
+    if (a.a_rows == 0) return fail(MI_EXPERTS_ERR_INVALID, "%s: a has no rows for row_ids", who);
+    if (!a.a || !a.a_scale || !a.b || !a.b_scale || !a.out || (a.num_experts && !a.expert_offsets))
         return fail(MI_EXPERTS_ERR_INVALID, "%s: NULL pointer argument", who);
     if (!aligned(a.a_scale, 4) || !aligned(a.b_scale, 4) || !aligned(a.out, size_of(a.out_dtype)) ||
         !aligned(a.bias, a.bias ? size_of(a.bias_dtype) : 1) || !aligned(a.expert_offsets, 4) ||

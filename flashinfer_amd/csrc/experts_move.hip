@@ -31,9 +31,10 @@ __device__ __forceinline__ int token_in_group(int tx_log) {
     return ONE ? __builtin_amdgcn_readfirstlane(t) : t;
 }
 
-inline unsigned blocks_for(int64_t T, int tx_log) {
-    const int64_t b = (T + (THREADS >> tx_log) - 1) / (THREADS >> tx_log);
-    return (unsigned)(b < MAX_BLOCKS ? b : MAX_BLOCKS);
+// Workgroups over T tokens and `chunks` column chunks, fewer than 2^32 threads.
+inline dim3 grid_for(int64_t T, int tx_log, int64_t chunks) {
+    const int64_t b = (T + (THREADS >> tx_log) - 1) / (THREADS >> tx_log), most = ((int64_t)1 << 23) / chunks;
+    return dim3((unsigned)(b < most ? b : most), (unsigned)chunks);
 }
 
 // Rows that all together exceed the 256 MB of the last cache are stored past
@@ -91,7 +92,7 @@ hipError_t launch_permute(const void* x, int64_t x_stride, int64_t T, int k, int
         typedef decltype(unit) V;
         const int64_t vectors = row_bytes / (int64_t)sizeof(V);
         const int tx_log = lanes_log(vectors);
-        const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
+        const dim3 grid = grid_for(T, tx_log, (vectors + (1 << tx_log) - 1) >> tx_log);
         const bool stream = streams(T * k * row_bytes);
         const auto kernel = tx_log >= 6 ? (stream ? permute_kernel<V, true, true> : permute_kernel<V, true, false>)
                                         : (stream ? permute_kernel<V, false, true> : permute_kernel<V, false, false>);
@@ -251,7 +252,7 @@ hipError_t launch_unpermute(int dtype, const void* rows, int64_t rows_stride, in
         constexpr int N = decltype(width)::value;
         const int64_t vectors = (H + N - 1) / N;
         const int tx_log = lanes_log(vectors);
-        const dim3 grid(blocks_for(T, tx_log), (unsigned)((vectors + (1 << tx_log) - 1) >> tx_log));
+        const dim3 grid = grid_for(T, tx_log, (vectors + (1 << tx_log) - 1) >> tx_log);
         const auto kernel = weights ? (tx_log >= 6 ? unpermute_kernel<E, N, true, true> : unpermute_kernel<E, N, true, false>)
                                     : (tx_log >= 6 ? unpermute_kernel<E, N, false, true> : unpermute_kernel<E, N, false, false>);
         hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, s, (const E*)rows, rows_stride, T, k, H, row_of_slot,
@@ -277,7 +278,7 @@ hipError_t launch_unpermute_backward(int dtype, const void* grad, int64_t grad_s
             tx_log >= 6
                 ? (stream ? unpermute_backward_kernel<E, N, true, true> : unpermute_backward_kernel<E, N, true, false>)
                 : (stream ? unpermute_backward_kernel<E, N, false, true> : unpermute_backward_kernel<E, N, false, false>);
-        hipLaunchKernelGGL(kernel, dim3(blocks_for(T, tx_log)), dim3(THREADS), 0, s, (const E*)grad, grad_stride,
+        hipLaunchKernelGGL(kernel, grid_for(T, tx_log, 1), dim3(THREADS), 0, s, (const E*)grad, grad_stride,
                            (const E*)rows, rows_stride, T, k, H, row_of_slot, num_rows, weights, (E*)grad_rows,
                            grad_rows_stride, (int)zero_rest, grad_weights, tx_log);
         return hipGetLastError();

@@ -119,7 +119,7 @@ def test_int8_matmul_refuses():
             (good, dict(expert_offsets=P), "grouped"), (good, dict(num_experts=-1), "num_experts"),
             (good, dict(N=1 << 29, rows=1 << 20, a_rows=1 << 20, out_stride=1 << 29), "too many"),
             (good, dict(a_rows=-1, rows=-1), "size"), (grouped, dict(expert_offsets=None), "NULL"),
-            (grouped, dict(bias=P), "bias"), (grouped, dict(num_experts=1025), "num_experts")]:
+            (grouped, dict(a_rows=0, row_ids=P), "no rows"), (grouped, dict(bias=P), "bias"), (grouped, dict(num_experts=1025), "num_experts")]:
         a = Args(**dict(base, **change))
         rc, msg = call("mi_experts_int8_matmul", [ctypes.POINTER(Args), ptr], [ctypes.byref(a), None])
         assert rc == 1 and word in msg, (change, rc, msg)

@@ -49,7 +49,7 @@ def plan_of(ids, E, offset):
 SORTS = [  # T, k, G, E, offset
     (0, 8, 8, 8, 0), (1, 1, 1, 1, 0), (1, 8, 256, 256, 0), (1, 8, 256, 32, 224), (7, 3, 16, 16, 0),
     (64, 8, 256, 32, 64), (65, 1, 5, 5, 0), (333, 6, 128, 16, 16), (1000, 8, 256, 256, 0),
-    (1024, 8, 64, 8, 8), (1025, 8, 1024, 1024, 0), (5000, 7, 256, 255, 1), (3001, 64, 1024, 1000, 3),
+    (1024, 8, 64, 8, 8), (512, 8, 1024, 1024, 0), (513, 8, 1024, 1024, 0), (1025, 8, 1024, 1024, 0), (5000, 7, 256, 255, 1), (3001, 64, 1024, 1000, 3),
     (70000, 8, 256, 32, 32)]
 
 
@@ -330,6 +330,8 @@ def test_refusals():
         (ValueError, lambda: fa.permute(x, plan, out=rows[:11])),
         (TypeError, lambda: fa.permute(x, plan, out=rows.float())),
         (ValueError, lambda: fa.permute(x, plan, out=rows[:1].expand(12, 16))),
+        (ValueError, lambda: fa.permute(rows[:6], plan, out=rows)),
+        (ValueError, lambda: fa.unpermute(rows, plan, out=rows[6:])),
         (ValueError, lambda: fa.permute(leaf, plan, out=rows)),
         (TypeError, lambda: fa.permute(x.double().requires_grad_(), plan)),
         (TypeError, lambda: fa.unpermute(rows.double(), plan)),
@@ -350,6 +352,17 @@ def test_refusals():
     g = torch.ones_like(y).requires_grad_()
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y, leaf, g, create_graph=True)
+
+
+def test_long_rows():
+    """Rows of 8 MB in single bytes: more column chunks than a launch takes with many tokens."""
+    T, H = 600, 1 << 23
+    x = torch.zeros(1, H, dtype=torch.uint8, device="cuda").random_(0, 256)
+    plan = fa.sort_experts(torch.zeros(T, 1, dtype=torch.int32, device="cuda"), 1)
+    out = torch.zeros(T, H + 1, dtype=torch.uint8, device="cuda")
+    fa.permute(x.expand(T, H), plan, out=out[:, 1:])
+    assert torch.equal(out[0, 1:], x[0]) and torch.equal(out[T // 2, 1:], x[0]) and torch.equal(out[-1, 1:], x[0])
+    assert not out[:, 0].any()
 
 
 def test_no_tokens():

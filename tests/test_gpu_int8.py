@@ -251,6 +251,65 @@ def test_offsets_past_32_bits():
     assert not y[:2].any()
 
 
+def test_gathered_rows_past_32_bits():
+    """Tokens whose rows lie more than 2^32 bytes into a."""
+    M, K, N = 140000, 32768, 64
+    a = torch.zeros(M, K, dtype=torch.int8, device="cuda")
+    a[-50:] = _ints((50, K), 1)
+    b, sa, sb = _ints((2, N, K), 2), _scales(M, 3), _scales((2, N), 4)
+    ids = torch.arange(M - 50, M, device="cuda", dtype=torch.int32).flip(0)
+    offs = torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda")
+    y = fa.int8_grouped_matmul(a, sa, b, sb, offs, row_ids=ids)
+    for e, rows in enumerate((slice(0, 20), slice(20, 50))):
+        _check(y[rows], _exact(a[ids[rows].long()], b[e]), sa[ids[rows].long()], sb[e])
+
+
+def test_copied_product_in_graphs():
+    """Large products of rows at any address copy them to a workspace: two
+    captured graphs, replayed in turn, keep theirs apart."""
+    M, N, K = 2048, 2112, 4111
+    made = []
+    for seed in (1, 2):
+        a, b, sa, sb = _ints((M, K), seed), _ints((N, K), seed + 2), _scales(M, 3), _scales(N, 4)
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            fa.int8_matmul(a, sa, b, sb)
+        torch.cuda.current_stream().wait_stream(st)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = fa.int8_matmul(a, sa, b, sb)
+        made.append((graph, a, b, sa, sb, y))
+    for rep in range(3):
+        for n, (_, a, *_) in enumerate(made):
+            a.copy_(_ints((M, K), 10 * rep + n))
+        for graph, *_ in made:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, a, b, sa, sb, y in made:
+            assert torch.equal(y, fa.int8_matmul(a, sa, b, sb))
+    _check(y, _exact(a, b), sa, sb)
+
+
+def test_buffers_are_apart_and_counted_as_written():
+    a, b, sa, sb = _ints((64, 64), 1), _ints((64, 64), 2), _scales(64, 3), _scales(64, 4)
+    big = torch.zeros(64, 128, dtype=torch.float32, device="cuda")
+    as_int8 = big.view(torch.int8)  # [64, 512]
+    with pytest.raises(ValueError, match="shares memory"):
+        fa.int8_matmul(as_int8[:, :64], sa, b, sb, out=big[:, :64])
+    fa.int8_matmul(as_int8[:, 256:320], sa, b, sb, out=big[:, :64])  # other columns of one buffer
+    x = torch.randn(4, 64, device="cuda")
+    with pytest.raises(ValueError, match="shares memory"):
+        fa.quantize_int8(x, q=x.view(torch.int8)[:, :64])
+    buf = torch.ones(64, 64, dtype=torch.bfloat16, device="cuda")
+    p = torch.randn(64, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    y = (p * buf).sum()  # keeps buf for its gradient
+    with torch.no_grad():
+        fa.int8_matmul(a, sa, b, sb, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
 @pytest.mark.parametrize("T", [1, 3, 40, 700])
 def test_expert_layer_in_int8(T):
     """route, sort, gathered product, SwiGLU and quantiser, second product,
@@ -361,6 +420,7 @@ def test_refusals():
         (TypeError, lambda: fa.int8_grouped_matmul(a, sa, w, sw, offs.long())),
         (TypeError, lambda: fa.int8_grouped_matmul(a, sa, w, sw, offs, row_ids=offs.long())),
         (ValueError, lambda: fa.int8_grouped_matmul(a, sa, w, sw[0], offs)),
+        (ValueError, lambda: fa.int8_grouped_matmul(a[:0], sa[:0], w, sw, offs, row_ids=offs)),
         (TypeError, lambda: fa.quantize_int8(x.double())),
         (ValueError, lambda: fa.quantize_int8(x[0])),
         (ValueError, lambda: fa.quantize_int8(x.clone().requires_grad_())),
