@@ -168,7 +168,7 @@ hipError_t launch_int8_tile(const Int8Call& p, int out_dtype, Int8Tile tile, boo
         case Int8Tile::T32x32: return launch<32, 32, 4, 4>(p, out_dtype, vec, s);
         case Int8Tile::T32x64: return launch<32, 64, 3, 4>(p, out_dtype, vec, s);
         case Int8Tile::T64x64_K2: return launch<64, 64, 3, 2>(p, out_dtype, vec, s);
-        case Int8Tile::T64x64: return launch<64, 64, 4, 1>(p, out_dtype, vec, s);
+        case Int8Tile::T64x64: return launch<64, 64, 3, 1>(p, out_dtype, vec, s);
         case Int8Tile::T64x128_K2: return launch<64, 128, 3, 2>(p, out_dtype, vec, s);
         case Int8Tile::T64x128: return launch<64, 128, 3, 1>(p, out_dtype, vec, s);
         case Int8Tile::T128x128_K2: return launch<128, 128, 2, 2>(p, out_dtype, vec, s);
