@@ -5,7 +5,12 @@
 // k rows that belong to it are written (or gathered) from there, so the
 // smaller side of the traffic crosses HBM once and no row index has to be
 // inverted. The sums over a token's slots and over a row's columns run in
-// fp32 in a fixed order; no atomics. All are bound by HBM.
+// fp32 in a fixed order; no atomics.
+//
+// All are bound by HBM. On MI355X, where a large copy reaches 4.7 TB/s, 8192
+// tokens x 8 rows of 7168 bf16: permute 218 us (4.9 TB/s), unpermute 195 us
+// (5.4), its gradients 400 us (5.0); one token: 2.8 us. Rows are read past the
+// caches (unpermute 235 us without).
 //
 // tx = 2^tx_log lanes share a token (as many as its row has vectors, at most
 // a workgroup), so short rows still fill the waves. From 64 lanes on a wave has
@@ -39,7 +44,11 @@ inline dim3 grid_for(int64_t T, int tx_log, int64_t chunks) {
 
 // Rows that all together exceed the 256 MB of the last cache are stored past
 // it: they would be gone before their reader comes, and what they push out has
-// to be written back meanwhile.
+// to be written back meanwhile (permute and its gradient, 3001 x 6 rows of
+// 4096 fp32: 53 + 100 us cached, 57 + 62 past it; 8192 x 8 of 7168 bf16 184 +
+// 258 against 219 + 192). Smaller ones are stored faster into it (8000 rows of 7168
+// bf16 18.5 us, 23.5 past it; the gradients of 3001 x 6 of 4096 fp16 53 and 57)
+// and stay for their reader.
 inline bool streams(int64_t bytes) { return bytes > (int64_t)256 << 20; }
 
 // Rows of slots j0 .. j0 + KG - 1 of token t (-1 past the k of it), all loaded

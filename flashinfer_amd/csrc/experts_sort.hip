@@ -12,7 +12,10 @@
 //
 // Up to SMALL slots one workgroup does it all. Beyond, one launch counts the
 // buckets of at most 256 chunks, and a second one places them: each workgroup
-// sums the counts of the chunks before its own, which are in L2.
+// sums the counts of the chunks before its own, which are in L2. What bounds
+// it is the latency of a few dependent passes, not its 12 bytes a slot: 8
+// slots 4.2 us, 4096 9.2, 8000 in two launches 9.1 (21 in one workgroup),
+// 65536 13.5, a million 46.
 #include "experts_common.hpp"
 
 namespace miexp {

@@ -7,6 +7,11 @@
 // What a small tile costs is the length of that chain (wait, barrier, LDS
 // reads, a few MFMAs), so sharing K shortens it and gives each SIMD a wave to
 // run while another one waits. The groups' integer sums meet in LDS at the end.
+// Against N = 4096, K = 7168 (29 MB of weights, 6 us at 5 TB/s): M = 1 and 64
+// 8.3 and 8.9 us with 32 x 32 tiles and K in four (64 x 64 with K in two 14 and
+// 15, whole 17), 128 11.8 (32 x 64, four), 256 16.7 (64 x 64, two; 18.8 whole),
+// 512 23.8 (64 x 128, two; 26.2 whole), 1024 35.9 (128 x 128, two; 40.4 whole),
+// 2048 59 (128 x 128 whole, two workgroups to a CU, 2.0 POP/s).
 //
 // LDS rows are 128 bytes, 16-byte chunk c of row r at position c ^ swzq(r).
 // Copies past K read zeros; rows past the tile repeat its last one and are not

@@ -24,7 +24,21 @@
 // one group stores its results while the other still multiplies.
 //
 // Results go through LDS, a wave's 16 rows at a time, so that stores cover
-// whole 128-byte lines.
+// whole 128-byte lines (8192 x 8192 x 1024: 86 us, 121 with a store per MFMA
+// tile and a workgroup per tile).
+//
+// 8192 x 4096 x 7168 185-189 us (2.6 POP/s; a loop of nothing but these MFMAs
+// on random data reaches 3.2, held by power), 4096 x 4096 x 7168 91 us. A step
+// takes about 3,300 cycles, 2,048 of them MFMA; the M0 slots, whose 64 KB of
+// LDS reads take longer than 32 MFMAs, make most of the rest. Experts' products
+// with few rows each wait for their weights instead: 8192 rows over 32 experts
+// of 7168 x 2048 180-200 us for 604 MB and 0.24 TOP.
+//
+// Measured and left out: four waves of 128 x 128 (a third fewer LDS reads, but
+// copies only half a step ahead: 245 us), phases by halves of K instead of rows
+// (evenly long, copies a step ahead: 230), reading the second halves during the
+// C phases (214), shares of tiles by cost or from a queue (no faster: tiles of
+// few rows cost as much as full ones, their weights).
 #include "int8_common.hpp"
 
 namespace miexp {

@@ -125,9 +125,11 @@ typedef struct mi_experts_int8_args {
     int32_t out_dtype;             /* MI_EXPERTS_* */
     int32_t bias_dtype;
     int32_t reserved;              /* must be 0 */
-    void* workspace;
+    void* workspace;               /* of the call below, 256-byte aligned; NULL where it says 0 */
     size_t workspace_bytes;
 } mi_experts_int8_args;
+/* 0 but for large dense products whose K is no multiple of 16: their rows are
+ * copied to aligned ones first. */
 size_t mi_experts_int8_workspace_size(int64_t rows, int64_t N, int64_t K, int32_t num_experts);
 int mi_experts_int8_matmul(const mi_experts_int8_args* args, void* stream);
 
