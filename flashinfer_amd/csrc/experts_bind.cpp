@@ -340,6 +340,7 @@ py::tuple quantize(const Tensor& x, bool swiglu, const OptTensor& num_rows, cons
         expect_device(*num_rows, "num_rows", x);
     }
     expect_no_grad(swiglu ? "swiglu_quantize_int8" : "quantize_int8", {&x});
+    if (scale_out) expect_no_grad(swiglu ? "swiglu_quantize_int8" : "quantize_int8", {&*scale_out});
     On on(x);
     const bool given_q = q_out && q_out->defined(), given_s = scale_out && scale_out->defined();
     const Tensor none, &count = num_rows ? *num_rows : none;

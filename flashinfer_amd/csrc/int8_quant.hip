@@ -24,7 +24,8 @@ constexpr float QUANT_FLOOR = 1e-10f;  // scale of an all-zero row: that of quan
 // -u log2(e) to twice the precision, the quotient a reciprocal and one Newton
 // step: within 6 * 2^-24 of the value, in half the instructions of a library
 // exponential and an IEEE division, which bound this kernel. Where 1 + exp(-u)
-// leaves the reciprocal's range, those are what is computed.
+// leaves the reciprocal's range, or u log2(e) that of fp32, those are what is
+// computed.
 template <int N>
 __device__ __forceinline__ void swiglu(float (&v)[N], const float (&u)[N]) {
     constexpr float L2E = 1.44269502f, L2E_LO = 1.92596299e-8f, LN2 = 0.693147182f;
@@ -35,7 +36,7 @@ __device__ __forceinline__ void swiglu(float (&v)[N], const float (&u)[N]) {
         const float hi = -u[i] * L2E, lo = fmaf(-u[i], L2E_LO, fmaf(-u[i], L2E, -hi));
         float x = __builtin_amdgcn_exp2f(hi);
         x = fmaf(x, lo * LN2, x);
-        far |= !(u[i] > -87.f);
+        far |= !(fabsf(u[i]) < 87.f);
         const float d = 1.f + x, rc = __builtin_amdgcn_rcpf(d), q = u[i] * rc;
         s[i] = fmaf(fmaf(-q, d, u[i]), rc, q);
     }

@@ -216,6 +216,23 @@ def test_swiglu_quantize(shape, dtype):
     assert bool(((q.to(F64) - v / want[:, None]).abs() <= 0.5 + 127 * 16.1 * U).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("K", [5, 64])
+def test_swiglu_of_extreme_gates(K, dtype):
+    """Gates up to the type's largest value; those below -90 give (next to) nothing."""
+    most = torch.finfo(dtype).max
+    gates = torch.tensor([most, most / 2, 3e4, 90.0, 87.0, 86.5, -86.5, -87.0, -90.0, -most], dtype=F64)
+    x = torch.empty(len(gates), 2 * K, dtype=F64).uniform_(-0.5, 0.5, generator=torch.Generator().manual_seed(1))
+    x[:, K] = gates
+    x = x.to(dtype).cuda()
+    q, s = fa.swiglu_quantize_int8(x)
+    v = x.to(F64)
+    v = v[:, K:] * torch.sigmoid(v[:, K:]) * v[:, :K]
+    want = v.abs().amax(dim=1) / 127.0
+    assert bool(((s.to(F64) - want).abs() <= 8 * U * want * 1.001).all())
+    assert bool(((q.to(F64) - v / want[:, None]).abs() <= 0.5 + 127 * 16.1 * U).all())
+
+
 def test_quantize_rows_in_use_and_poisoned_rows():
     x = torch.randn(10, 96, generator=_gen(1), device="cuda")
     n = torch.tensor([6], dtype=torch.int32, device="cuda")
@@ -429,6 +446,7 @@ def test_refusals():
         (ValueError, lambda: fa.quantize_int8(x, num_rows=offs)),
         (TypeError, lambda: fa.quantize_int8(x, q=x)),
         (ValueError, lambda: fa.quantize_int8(x, scale=sa[:2])),
+        (ValueError, lambda: fa.quantize_int8(x, scale=sa.clone().requires_grad_())),
     ]
     for n, (error, call) in enumerate(bad):
         with pytest.raises(error):
