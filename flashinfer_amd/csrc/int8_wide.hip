@@ -29,16 +29,20 @@
 //
 // 8192 x 4096 x 7168 185-189 us (2.6 POP/s; a loop of nothing but these MFMAs
 // on random data reaches 3.2, held by power), 4096 x 4096 x 7168 91 us. A step
-// takes about 3,300 cycles, 2,048 of them MFMA; the M0 slots, whose 64 KB of
-// LDS reads take longer than 32 MFMAs, make most of the rest. Experts' products
-// with few rows each wait for their weights instead: 8192 rows over 32 experts
-// of 7168 x 2048 180-200 us for 604 MB and 0.24 TOP.
+// takes about 3,300 cycles, 2,048 of them MFMA. No one part holds it: where the
+// whole takes 204 us, it is 178 without the copies, 188 without the LDS reads
+// and 140 without the MFMAs, so what is left is in the slots' ends. Experts'
+// products with few rows each are bound as much by their weights: 8192 rows
+// over 32 experts of 7168 x 2048 180-215 us for 604 MB and 0.24 TOP, 173
+// without the copies, 177 without the MFMAs.
 //
 // Measured and left out: four waves of 128 x 128 (a third fewer LDS reads, but
 // copies only half a step ahead: 245 us), phases by halves of K instead of rows
 // (evenly long, copies a step ahead: 230), reading the second halves during the
-// C phases (214), shares of tiles by cost or from a queue (no faster: tiles of
-// few rows cost as much as full ones, their weights).
+// C phases (214), 32 x 32 x 32 MFMAs (5 % faster by themselves; 228 against
+// 204), weights from memory into registers (neighbouring lanes read different
+// rows: 313 against 203), shares of tiles by cost or from a queue (no faster:
+// tiles of few rows cost as much as full ones, their weights).
 #include "int8_common.hpp"
 
 namespace miexp {
