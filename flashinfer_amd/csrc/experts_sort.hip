@@ -14,19 +14,23 @@
 // buckets of at most 256 chunks, and a second one places them: each workgroup
 // sums the counts of the chunks before its own, which are in L2. What bounds
 // it is the latency of a few dependent passes, not its 12 bytes a slot: 8
-// slots 4.2 us, 4096 9.2, 8000 in two launches 9.1 (21 in one workgroup),
-// 65536 13.5, a million 46.
+// slots 4.2 us, 2048 6.6, 4096 8.5 (9.1 in one workgroup), 8000 8.4 (21),
+// 65536 13.5, a million 47.
 #include "experts_common.hpp"
 
 namespace miexp {
 
-constexpr int64_t SMALL = 4096;
+constexpr int64_t SMALL = 3000;
 constexpr int64_t MAX_CHUNKS = 256;
-constexpr int CHUNK_MIN = 2048;
 
-__host__ __device__ inline int64_t chunk_len(int64_t slots) {
-    const int64_t per = (slots + MAX_CHUNKS - 1) / MAX_CHUNKS;
-    return per <= CHUNK_MIN ? CHUNK_MIN : (per + 1023) / 1024 * 1024;
+// Slots of a chunk. Short chunks shorten a wave's walk, many chunks the sums
+// over them: 16 to 20 of 512 or 1024 slots (8000 slots: 8.4 us, 9.5 in four;
+// 16384: 9.6 in 16, 10.7 in 32), 32 to 64 of 2048 to 4096 (65536: 13.5 in 32,
+// 18.4 in 16; 524288: 38 in 64, 43 in 256, 60 in 32), beyond 64 of 8192 up to 256.
+inline int64_t chunk_len(int64_t slots) {
+    int64_t len = 512;
+    while (len * (len < 1024 ? 20 : len < 2048 ? 32 : len < 8192 ? 64 : MAX_CHUNKS) < slots) len *= 2;
+    return len;
 }
 
 int64_t sort_chunks(int64_t slots) {

@@ -50,7 +50,7 @@ SORTS = [  # T, k, G, E, offset
     (0, 8, 8, 8, 0), (1, 1, 1, 1, 0), (1, 8, 256, 256, 0), (1, 8, 256, 32, 224), (7, 3, 16, 16, 0),
     (64, 8, 256, 32, 64), (65, 1, 5, 5, 0), (333, 6, 128, 16, 16), (1000, 8, 256, 256, 0),
     (1024, 8, 64, 8, 8), (512, 8, 1024, 1024, 0), (513, 8, 1024, 1024, 0), (1025, 8, 1024, 1024, 0), (5000, 7, 256, 255, 1), (3001, 64, 1024, 1000, 3),
-    (70000, 8, 256, 32, 32)]
+    (70000, 8, 256, 32, 32), (1500, 2, 64, 64, 0), (3001, 1, 64, 8, 8), (1281, 8, 256, 256, 0), (4097, 8, 1024, 1024, 0)]
 
 
 @pytest.mark.parametrize("case", SORTS, ids=str)
