@@ -356,15 +356,17 @@ py::tuple quantize(const Tensor& x, bool swiglu, const OptTensor& num_rows, cons
     }
     const auto opt = x.options().requires_grad(false);
     const bool cut = num_rows && num_rows->defined();
+    // rows past num_rows: the kernel's to clear if both buffers are new
+    const bool zero_rest = cut && !given_q && !given_s;
     auto fresh = [&](at::IntArrayRef shape, at::ScalarType t) {
-        return cut ? at::zeros(shape, opt.dtype(t)) : at::empty(shape, opt.dtype(t));
+        return cut && !zero_rest ? at::zeros(shape, opt.dtype(t)) : at::empty(shape, opt.dtype(t));
     };
     Tensor q = given_q ? *q_out : fresh({M, K}, at::kChar);
     Tensor scale = given_s ? *scale_out : fresh({M}, at::kFloat);
     if (M > 0) {
         const Tensor in = rows_of(x);
         check(mi_experts_quantize_int8(dtype, in.const_data_ptr(), row_stride(in), M, K, swiglu,
-                                       cut ? num_rows->const_data_ptr<int32_t>() : nullptr,
+                                       cut ? num_rows->const_data_ptr<int32_t>() : nullptr, zero_rest,
                                        q.mutable_data_ptr<int8_t>(), row_stride(q), scale.mutable_data_ptr<float>(),
                                        on.stream));
     }
@@ -434,8 +436,7 @@ Tensor int8_call(const Tensor& a, const Tensor& a_scale, const Tensor& b, const 
     }
     On on(a);
     const auto opt = a.options().requires_grad(false).dtype(out_type);
-    // rows that no expert has are not written by a grouped product
-    Tensor out = given ? *out_opt : grouped ? at::zeros({rows, N}, opt) : at::empty({rows, N}, opt);
+    Tensor out = given ? *out_opt : at::empty({rows, N}, opt);
     if (out.numel() == 0) return out;
     const Tensor ac = rows_of(a), as = a_scale.contiguous(), bs = b_scale.contiguous();
     const Tensor bc = rows_of(b);
@@ -466,6 +467,7 @@ Tensor int8_call(const Tensor& a, const Tensor& a_scale, const Tensor& b, const 
     c.b_expert_stride = grouped && E > 1 ? bc.stride(0) : 0;
     c.out_stride = row_stride(out);
     c.num_experts = (int32_t)E;
+    c.zero_rest = grouped && !given;
     const size_t need = mi_experts_int8_workspace_size(rows, N, K, (int32_t)E);
     Tensor ws;
     if (need) {

@@ -152,8 +152,9 @@ int mi_experts_unpermute_backward(int32_t dtype, const void* grad, int64_t grad_
 }
 
 int mi_experts_quantize_int8(int32_t dtype, const void* x, int64_t x_stride, int64_t num_rows_max,
-                             int64_t row_len, int32_t swiglu, const int32_t* num_rows, int8_t* q,
-                             int64_t q_stride, float* scale, void* stream) {
+                             int64_t row_len, int32_t swiglu, const int32_t* num_rows,
+                             int32_t zero_rest, int8_t* q, int64_t q_stride, float* scale,
+                             void* stream) {
     const char* who = "mi_experts_quantize_int8";
     g_last_error[0] = 0;
     if (!float_type(dtype)) return fail(MI_EXPERTS_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
@@ -167,7 +168,7 @@ int mi_experts_quantize_int8(int32_t dtype, const void* x, int64_t x_stride, int
     if (!aligned(x, size_of(dtype)) || !aligned(scale, 4) || !aligned(num_rows, 4))
         return fail(MI_EXPERTS_ERR_INVALID, "%s: misaligned pointer", who);
     return hip_status(who, launch_quantize(dtype, x, x_stride, num_rows_max, row_len, swiglu != 0, num_rows,
-                                           q, q_stride, scale, (hipStream_t)stream));
+                                           zero_rest != 0, q, q_stride, scale, (hipStream_t)stream));
 }
 
 size_t mi_experts_int8_workspace_size(int64_t rows, int64_t N, int64_t K, int32_t num_experts) {
@@ -180,7 +181,6 @@ int mi_experts_int8_matmul(const mi_experts_int8_args* args, void* stream) {
     g_last_error[0] = 0;
     if (!args) return fail(MI_EXPERTS_ERR_INVALID, "%s: args is NULL", who);
     const mi_experts_int8_args& a = *args;
-    if (a.reserved != 0) return fail(MI_EXPERTS_ERR_INVALID, "%s: reserved must be 0", who);
     if (!float_type(a.out_dtype) || (a.bias && !float_type(a.bias_dtype)))
         return fail(MI_EXPERTS_ERR_INVALID, "%s: unknown dtype", who);
     if (a.num_experts < 0 || a.num_experts > MI_EXPERTS_MAX_EXPERTS)

@@ -88,7 +88,7 @@ hipError_t launch_unpermute_backward(int dtype, const void* grad, int64_t grad_s
                                      const float* weights, void* grad_rows, int64_t grad_rows_stride,
                                      bool zero_rest, float* grad_weights, hipStream_t s);
 hipError_t launch_quantize(int dtype, const void* x, int64_t x_stride, int64_t M, int64_t K, bool swiglu,
-                           const int32_t* num_rows, int8_t* q, int64_t q_stride, float* scale,
+                           const int32_t* num_rows, bool zero_rest, int8_t* q, int64_t q_stride, float* scale,
                            hipStream_t s);
 hipError_t launch_int8_matmul(const mi_experts_int8_args& a, hipStream_t s);
 size_t int8_workspace(int64_t rows, int64_t N, int64_t K, int E);

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256 * KS) void int8_any_kernel(Int8Call p, int ntil
     static_assert((KS - 1) * BM * BN * 4 <= (int)sizeof(smem), "LDS budget");
     int e, nrows;
     int64_t row0;
-    if (!find_tile<BM>(p, blockIdx.x / ntiles, e, row0, nrows)) return;
+    if (!find_tile<BM>(p, blockIdx.x / ntiles, e, row0, nrows)) return zero_rest<T>(p, vec);
     const int n0 = (int)(blockIdx.x % ntiles) * BN;
     const int lane = threadIdx.x & 63, tid = threadIdx.x & 255;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -135,8 +135,8 @@ __global__ __launch_bounds__(256 * KS) void int8_any_kernel(Int8Call p, int ntil
         }
     }
     sum_groups<KS, MT, NT>(smem, ks, wave, acc);
-    if (ks > 0) return;
-    store_tiles<T>(p, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec, acc, scales);
+    if (ks == 0) store_tiles<T>(p, row0, nrows, wm * (BM / 2), n0 + wn * (BN / 2), vec, acc, scales);
+    zero_rest<T>(p, vec);
 }
 
 template <int BM, int BN, int KS>

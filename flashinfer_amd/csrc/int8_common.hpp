@@ -22,6 +22,7 @@ struct Int8Call {
     int64_t a_stride, b_stride, b_expert_stride, out_stride;
     int E;
     int bias_dtype;
+    int zero_rest;  // rows that no expert has get zeros
     int b_large;  // the weights exceed the 256 MB of the last cache
 };
 
@@ -208,6 +209,27 @@ __device__ __forceinline__ void store_tiles(const Int8Call& p, int64_t row0, int
 #pragma unroll
                 for (int v = 0; v < 4; ++v)
                     if (at + v < p.N) to[v] = (T)y[v];
+            }
+        }
+    }
+}
+
+// Zeros for the rows before the first expert's and behind the last one's, by
+// all workgroups of a launch once their tiles are done (8192 rows, all in use,
+// of 7168 x 2048 over 32 experts: 152 us with or without; a fill of the whole
+// result before the product took 30 more).
+template <class T>
+__device__ __forceinline__ void zero_rest(const Int8Call& p, bool vec) {
+    if (!p.zero_rest) return;
+    const int64_t first = clamped(p.offsets, 0, p.rows), end = max(first, clamped(p.offsets, p.E, p.rows));
+    for (int64_t i = blockIdx.x; i < first + p.rows - end; i += gridDim.x) {
+        T* to = reinterpret_cast<T*>(p.out) + (i < first ? i : end + i - first) * p.out_stride;
+        for (int n = threadIdx.x * 4; n < p.N; n += blockDim.x * 4) {
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            if (vec && n + 4 <= p.N) {
+                store<T, 4>(to + n, zero);
+            } else {
+                for (int v = n; v < min(n + 4, p.N); ++v) to[v] = (T)0.f;
             }
         }
     }

@@ -82,6 +82,7 @@ hipError_t launch_int8_matmul(const mi_experts_int8_args& a, hipStream_t s) {
     p.out_stride = a.out_stride;
     p.E = a.num_experts;
     p.bias_dtype = a.bias_dtype;
+    p.zero_rest = a.num_experts != 0 && a.zero_rest != 0;
     p.b_large = (a.num_experts ? a.num_experts : 1) * a.N * a.K > ((int64_t)256 << 20);
     if (int8_workspace(a.rows, a.N, a.K, a.num_experts)) {
         const int ld = (p.K + 15) / 16 * 16;

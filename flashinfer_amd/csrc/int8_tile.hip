@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256 * KS) void int8_tile_kernel(Int8Call p, int nti
     static_assert(sizeof(smem) <= 160 * 1024 && (KS - 1) * BM * BN * 4 <= (int)sizeof(smem), "LDS budget");
     Tiles x;
     const int mt = blockIdx.x / ntiles, n0 = (int)(blockIdx.x % ntiles) * BN;
-    if (!find_expert<BM>(p, mt, x)) return;
+    if (!find_expert<BM>(p, mt, x)) return zero_rest<T>(p, vec);
     const int64_t row0 = (int64_t)x.row + (int64_t)(mt - x.first) * BM;
     const int nrows = (int)min((int64_t)BM, x.end - row0);
     // Weights that no other row tile reads, of more than the last cache holds
@@ -156,6 +156,7 @@ __global__ __launch_bounds__(256 * KS) void int8_tile_kernel(Int8Call p, int nti
         tile_run<T, BM, BN, STAGES, KS, true>(p, smem, x.e, row0, nrows, n0, vec);
     else
         tile_run<T, BM, BN, STAGES, KS, false>(p, smem, x.e, row0, nrows, n0, vec);
+    zero_rest<T>(p, vec);
 }
 
 template <int BM, int BN, int STAGES, int KS>

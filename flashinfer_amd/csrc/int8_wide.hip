@@ -375,11 +375,13 @@ __global__ __launch_bounds__(512) void int8_wide_kernel(Int8Call p, int ntiles, 
     // each of the 8 XCDs (workgroup b runs on b % 8) takes one contiguous eighth of the order
     const int per_xcd = (total + 7) >> 3, xcd = blockIdx.x & 7;
     const int first = xcd * per_xcd + (blockIdx.x >> 3), end = min(total, (xcd + 1) * per_xcd);
-    if (first >= end) return;
-    if (threadIdx.x < 256)
-        wide_run<T, 0>(p, lds, ntiles, first, end, gridDim.x >> 3, vec16);
-    else
-        wide_run<T, 1>(p, lds, ntiles, first, end, gridDim.x >> 3, vec16);
+    if (first < end) {
+        if (threadIdx.x < 256)
+            wide_run<T, 0>(p, lds, ntiles, first, end, gridDim.x >> 3, vec16);
+        else
+            wide_run<T, 1>(p, lds, ntiles, first, end, gridDim.x >> 3, vec16);
+    }
+    zero_rest<T>(p, vec16);
 }
 
 // K > 128: two steps at least.

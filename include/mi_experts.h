@@ -93,18 +93,20 @@ int mi_experts_unpermute_backward(int32_t dtype, const void* grad, int64_t grad_
  * first silu(x[row_len:]) * x[:row_len] in fp32 (the layer's SwiGLU,
  * solution/triton/kernel.py:297-330). A row that holds a NaN or an infinity
  * gets a scale that is not finite and zeros, so its products are NaN. With
- * num_rows (device int32, may be NULL) rows at and past it are left as they
- * are. x_stride, q_stride in elements. */
+ * num_rows (device int32, may be NULL) rows at and past it get zeros (and a
+ * scale of 0) with zero_rest, else they are left as they are. x_stride,
+ * q_stride in elements. */
 int mi_experts_quantize_int8(int32_t dtype, const void* x, int64_t x_stride, int64_t num_rows_max,
-                             int64_t row_len, int32_t swiglu, const int32_t* num_rows, int8_t* q,
-                             int64_t q_stride, float* scale, void* stream);
+                             int64_t row_len, int32_t swiglu, const int32_t* num_rows,
+                             int32_t zero_rest, int8_t* q, int64_t q_stride, float* scale,
+                             void* stream);
 
 /* out[m, n] = (sum_k a[m, k] * b[n, k]) * a_scale[m] * b_scale[n] + bias[n],
  * the sum exact in int32, the rest in fp32, rounded once to out's type.
  * num_experts = 0: b [N, K], a [M, K], out [M, N]. Else b [E, N, K], b_scale
  * [E, N], out row m (m < rows) has the expert whose [expert_offsets[e],
- * expert_offsets[e+1]) holds it, and rows that no expert has are left as they
- * are. row_ids (int32 [rows], may be NULL): row m of the product is row
+ * expert_offsets[e+1]) holds it, and rows before the first expert's and behind
+ * the last one's are zeroed with zero_rest, else left as they are. row_ids (int32 [rows], may be NULL): row m of the product is row
  * row_ids[m] of a and of a_scale; an id outside [0, a_rows) gives NaN rows.
  * Offsets are clamped to [0, rows]. Any strides (in elements) and alignment;
  * 16-byte ones of a and b are fast. */
@@ -124,7 +126,7 @@ typedef struct mi_experts_int8_args {
     int32_t num_experts;           /* 0: dense */
     int32_t out_dtype;             /* MI_EXPERTS_* */
     int32_t bias_dtype;
-    int32_t reserved;              /* must be 0 */
+    int32_t zero_rest;             /* grouped products */
     void* workspace;               /* of the call below, 256-byte aligned; NULL where it says 0 */
     size_t workspace_bytes;
 } mi_experts_int8_args;

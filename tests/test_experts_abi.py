@@ -91,17 +91,17 @@ def test_moves_refuse():
 
 @cpu_only
 def test_quantize_refuses():
-    types = [i32, ptr, i64, i64, i64, i32, ptr, ptr, i64, ptr, ptr]
-    refused("mi_experts_quantize_int8", types, [1, P, 64, 16, 64, 0, None, P, 64, P, None], [
-        (0, 7, "dtype"), (1, None, "NULL"), (7, None, "NULL"), (9, None, "NULL"), (1, P + 2, "misaligned"),
-        (8, 63, "stride"), (2, -1, "stride"), (4, 0, "row length"), (3, -1, "rows"), (3, 1 << 31, "rows")])
+    types = [i32, ptr, i64, i64, i64, i32, ptr, i32, ptr, i64, ptr, ptr]
+    refused("mi_experts_quantize_int8", types, [1, P, 64, 16, 64, 0, None, 1, P, 64, P, None], [
+        (0, 7, "dtype"), (1, None, "NULL"), (8, None, "NULL"), (10, None, "NULL"), (1, P + 2, "misaligned"),
+        (9, 63, "stride"), (2, -1, "stride"), (4, 0, "row length"), (3, -1, "rows"), (3, 1 << 31, "rows")])
 
 
 class Args(ctypes.Structure):
     _fields_ = ([(n, ptr) for n in ("a", "a_scale", "b", "b_scale", "bias", "out", "expert_offsets", "row_ids")]
                 + [(n, i64) for n in ("a_rows", "rows", "N", "K", "a_stride", "b_stride", "b_expert_stride",
                                       "out_stride")]
-                + [(n, i32) for n in ("num_experts", "out_dtype", "bias_dtype", "reserved")]
+                + [(n, i32) for n in ("num_experts", "out_dtype", "bias_dtype", "zero_rest")]
                 + [("workspace", ptr), ("workspace_bytes", size)])
 
 
@@ -115,7 +115,7 @@ def test_int8_matmul_refuses():
             (good, dict(a_scale=None), "NULL"), (good, dict(b_scale=P + 1), "misaligned"), (good, dict(K=0), "K 0"),
             (good, dict(K=131072), "131072"), (good, dict(rows=5), "rows"), (good, dict(out_stride=7), "stride"),
             (good, dict(out_dtype=5), "dtype"), (good, dict(bias=P, bias_dtype=5), "dtype"),
-            (good, dict(reserved=1), "reserved"), (good, dict(row_ids=P), "grouped"),
+            (good, dict(row_ids=P), "grouped"),
             (good, dict(expert_offsets=P), "grouped"), (good, dict(num_experts=-1), "num_experts"),
             (good, dict(N=1 << 29, rows=1 << 20, a_rows=1 << 20, out_stride=1 << 29), "too many"),
             (good, dict(a_rows=-1, rows=-1), "size"), (grouped, dict(expert_offsets=None), "NULL"),

@@ -136,6 +136,49 @@ def test_grouped(case, dtype):
     assert torch.equal(buf[:lo], y[:lo]) and bool((buf[lo:] == 9).all())
 
 
+def _leave_behind(like):
+    """A freed block of the result's size that holds no zeros, for the next result to get."""
+    torch.full_like(like, 9)
+
+
+@pytest.mark.parametrize("tile", range(9))
+@pytest.mark.parametrize("shape", [(264, 400), (130, 515)], ids=str)
+def test_rows_without_an_expert_are_zeros(tile, shape, monkeypatch):
+    """Those behind the last expert's, and those before the first one's."""
+    monkeypatch.setenv("MI_INT8_TILE", str(tile))
+    N, K = shape
+    for offs, R in (([3, 3, 10, 300], 340), ([0, 0, 0, 0], 70), ([70, 70, 70, 70], 70), ([0, 1, 1, 1], 1)):
+        offs = torch.tensor(offs, dtype=torch.int32, device="cuda")
+        a, b, sa, sb = _ints((R, K), 1), _ints((3, N, K), 2), _scales(R, 3), _scales((3, N), 4)
+        buf = torch.full((R, N), 9.0, dtype=torch.bfloat16, device="cuda")
+        fa.int8_grouped_matmul(a, sa, b, sb, offs, out=buf)
+        _leave_behind(buf)
+        y = fa.int8_grouped_matmul(a, sa, b, sb, offs)
+        first, end = int(offs[0]), int(offs[-1])
+        assert torch.equal(y[first:end], buf[first:end])
+        assert not y[:first].any() and not y[end:].any()
+        assert bool((buf[:first] == 9).all()) and bool((buf[end:] == 9).all())
+
+
+@pytest.mark.parametrize("K", [33, 96, 2048, 5000])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_quantize_clears_rows_past_those_in_use(K, swiglu):
+    f = fa.swiglu_quantize_int8 if swiglu else fa.quantize_int8
+    M = 700
+    x = torch.randn(M, K * (1 + swiglu), generator=_gen(1), device="cuda").bfloat16()
+    q0, s0 = f(x)
+    for n in (-5, 0, 1, 699, 700, 5000):
+        count = torch.tensor([n], dtype=torch.int32, device="cuda")
+        _leave_behind(q0), _leave_behind(s0)
+        q, s = f(x, num_rows=count)
+        n = min(max(n, 0), M)
+        assert torch.equal(q[:n], q0[:n]) and torch.equal(s[:n], s0[:n])
+        assert not q[n:].any() and not s[n:].any()
+        s2 = torch.full_like(s0, 9)  # one buffer passed in, one new
+        q2, _ = f(x, num_rows=count, scale=s2)
+        assert torch.equal(q2, q) and torch.equal(s2[:n], s0[:n]) and bool((s2[n:] == 9).all())
+
+
 # the tiles of csrc/int8_common.hpp, each at sizes that end inside it
 @pytest.mark.parametrize("tile", range(9))
 @pytest.mark.parametrize("shape", [(1, 8, 144), (70, 90, 272), (130, 264, 2048), (259, 515, 1040), (300, 40, 7),
