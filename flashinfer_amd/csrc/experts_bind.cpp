@@ -10,6 +10,7 @@
 //
 // Built with g++ against torch's headers (no device code here).
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -131,6 +132,26 @@ void no_grad_out(const char* what, bool needs, const OptTensor& out) {
                       what, "(): out= takes no part in autograd; call it without out, or under torch.no_grad()");
 }
 
+// A tangent of forward-mode differentiation. It comes without requires_grad
+// and is there under torch.no_grad(), too.
+bool has_tangent(const Tensor& t) {
+    return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
+}
+
+// The results carry no tangents: inputs whose tangent would be lost, and
+// destinations that would keep a wrong one, are refused.
+void expect_no_tangent(const char* what, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_VALUE(!has_tangent(*t), what,
+                          "() has no forward-mode derivative and got a tensor with a tangent: detach it");
+}
+
+// An optional tensor, undefined if there is none.
+const Tensor& or_none(const OptTensor& t) {
+    static const Tensor none;
+    return t ? *t : none;
+}
+
 // ---------------------------------------------------------------- sorting
 
 py::tuple sort_experts(const Tensor& topk_ids, int64_t num_experts, int64_t expert_offset) {
@@ -215,6 +236,7 @@ struct PermuteFn : torch::autograd::Function<PermuteFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "permute() has no second derivative (create_graph=True)");
+        TORCH_CHECK(!has_tangent(grads[0]), "permute() has no second derivative (a gradient with a tangent)");
         const auto saved = ctx->get_saved_variables();
         const Plan p = plan_of(saved[0], saved[1], grads[0]);
         return {unpermute_new(grads[0], p, Tensor()), Tensor(), Tensor()};
@@ -223,6 +245,7 @@ struct PermuteFn : torch::autograd::Function<PermuteFn> {
 
 Tensor permute(const Tensor& hidden, const Tensor& offsets, const Tensor& row_of_slot, const OptTensor& out) {
     expect_dim(hidden, "hidden", 2);
+    expect_no_tangent("permute", {&hidden, &or_none(out)});
     expect_gpu(hidden, "hidden");
     const Plan p = plan_of(offsets, row_of_slot, hidden);
     TORCH_CHECK_VALUE(hidden.size(0) == p.T, "hidden has ", hidden.size(0), " tokens, the plan ", p.T);
@@ -261,6 +284,7 @@ struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "unpermute() has no second derivative (create_graph=True)");
+        TORCH_CHECK(!has_tangent(grads[0]), "unpermute() has no second derivative (a gradient with a tangent)");
         const auto saved = ctx->get_saved_variables();
         On on(grads[0]);
         const Tensor g = rows_of(grads[0]);
@@ -283,6 +307,7 @@ struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
 Tensor unpermute(const Tensor& rows, const Tensor& offsets, const Tensor& row_of_slot, const OptTensor& weights,
                  const OptTensor& out) {
     expect_dim(rows, "rows", 2);
+    expect_no_tangent("unpermute", {&rows, &or_none(weights), &or_none(out)});
     expect_gpu(rows, "rows");
     const int dtype = float_dtype(rows, "rows");
     const Plan p = plan_of(offsets, row_of_slot, rows);
@@ -329,6 +354,7 @@ py::tuple quantize(const Tensor& x, bool swiglu, const OptTensor& num_rows, cons
                    const OptTensor& scale_out) {
     expect_dim(x, "x", 2);
     const int dtype = float_dtype(x, "x");
+    expect_no_tangent(swiglu ? "swiglu_quantize_int8" : "quantize_int8", {&x, &or_none(scale_out)});
     expect_gpu(x, "x");
     const int64_t M = x.size(0), C = x.size(1);
     TORCH_CHECK_VALUE(!swiglu || C % 2 == 0, "x must have 2 I columns, got ", C);
@@ -384,6 +410,8 @@ Tensor int8_call(const Tensor& a, const Tensor& a_scale, const Tensor& b, const 
     expect_type(b, "b", at::kChar);
     expect_type(a_scale, "a_scale", at::kFloat);
     expect_type(b_scale, "b_scale", at::kFloat);
+    expect_no_tangent(grouped ? "int8_grouped_matmul" : "int8_matmul",
+                      {&a_scale, &b_scale, &or_none(bias), &or_none(out_opt)});
     expect_gpu(a, "a");
     const int64_t M = a.size(0), K = a.size(1), E = grouped ? b.size(0) : 0, N = b.size(-2);
     TORCH_CHECK_VALUE(b.size(-1) == K, "b must have ", K, " columns as a has, got shape ", b.sizes());

@@ -4,8 +4,9 @@
 token side alone, for experts of a caller's own: ``sort_experts`` places every
 (token, expert) slot of a routing at a row, ``permute`` lays the tokens' rows
 out in that order, and ``unpermute`` brings the experts' rows back to their
-tokens, weighted and summed. ``permute`` and ``unpermute`` are differentiable;
-the reference has neither (its sort and combine serve its one entry point,
+tokens, weighted and summed. ``permute`` and ``unpermute`` are differentiable
+(once, in reverse mode; tensors with a forward-mode tangent are refused); the
+reference has neither (its sort and combine serve its one entry point,
 solution/triton/kernel.py:460-505, :337-368).
 
 Everything runs on torch's current stream with no host synchronisation, and

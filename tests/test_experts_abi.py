@@ -151,3 +151,33 @@ def test_no_cpu_path():
         fa.int8_matmul(x, s, q, s)
     with pytest.raises(TypeError):
         fa.permute([1], plan)
+
+
+def test_tangents_are_refused():
+    """A dual tensor does not require a gradient, so its tangent would be lost
+    without a word; one that autograd was told to leave alone may go on."""
+    import torch.autograd.forward_ad as fwd
+    ids = torch.zeros(2, 3, dtype=torch.int32)
+    plan = fa.ExpertPlan(torch.zeros(5, dtype=torch.int32), torch.zeros(6, dtype=torch.int32), ids)
+    x, rows, w = torch.zeros(2, 16), torch.zeros(6, 16), torch.zeros(2, 3)
+    q, b, s = torch.zeros(2, 16, dtype=torch.int8), torch.zeros(1, 2, 16, dtype=torch.int8), torch.ones(2)
+    offs = torch.zeros(2, dtype=torch.int32)
+    calls = [(x, lambda t: fa.permute(t, plan)), (rows, lambda t: fa.permute(x, plan, out=t)),
+             (rows, lambda t: fa.unpermute(t, plan)), (w, lambda t: fa.unpermute(rows, plan, t)),
+             (x, lambda t: fa.unpermute(rows, plan, out=t)), (x, fa.quantize_int8), (x, fa.swiglu_quantize_int8),
+             (s, lambda t: fa.quantize_int8(x, scale=t)), (s, lambda t: fa.int8_matmul(q, t, q, s)),
+             (s, lambda t: fa.int8_matmul(q, s, q, t)), (s, lambda t: fa.int8_matmul(q, s, q, s, bias=t)),
+             (x, lambda t: fa.int8_matmul(q, s, q, s, out=t)),
+             (s, lambda t: fa.int8_grouped_matmul(q, t, b, s[None], offs)),
+             (s, lambda t: fa.int8_grouped_matmul(q, s, b, t[None], offs))]
+    with fwd.dual_level():
+        for n, (t, call) in enumerate(calls):
+            dual = fwd.make_dual(t, torch.ones_like(t))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                    call(dual)
+                    print("not refused:", n)
+            with pytest.raises(ValueError, match="no CPU path"):
+                call(dual.detach())
+            with torch.inference_mode(), pytest.raises(ValueError, match="no CPU path"):
+                call(dual)

@@ -375,3 +375,19 @@ def test_no_tokens():
     y = fa.unpermute(rows, plan, w)
     gx, gw = torch.autograd.grad(y.sum(), (x, w))
     assert gx.shape == (0, 64) and gw.shape == (0, 4)
+
+
+def test_gradients_with_tangents_are_refused():
+    """Forward over backward: a gradient's tangent would be lost on its way to the leaves."""
+    import torch.autograd.forward_ad as fwd
+    plan = fa.sort_experts(ids_of(6, 2, 4, 1).cuda(), 4)
+    x, rows = torch.ones(6, 16, device="cuda", requires_grad=True), torch.ones(12, 16, device="cuda", requires_grad=True)
+    w = torch.ones(6, 2, device="cuda", requires_grad=True)
+    for y, leaves in ((fa.permute(x, plan), (x,)), (fa.unpermute(rows, plan, w), (rows, w))):
+        g = torch.ones_like(y)
+        with fwd.dual_level():
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad(y, leaves, fwd.make_dual(g, g), retain_graph=True)
+            with pytest.raises(ValueError, match="forward-mode"):
+                fa.permute(fwd.make_dual(x, torch.ones_like(x)), plan)
+        assert all(bool((t == 2 if t is x else t >= 1).all()) for t in torch.autograd.grad(y, leaves, g))
