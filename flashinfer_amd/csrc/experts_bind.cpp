@@ -75,8 +75,13 @@ void expect_device(const Tensor& t, const char* name, const Tensor& like) {
     TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", expected ", like.device());
 }
 
+// Kernels read memory as it is: a view whose sign torch changes only when it is
+// read (the imaginary part of a conjugate) is copied.
+Tensor dense(const Tensor& t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
+
 // Rows of consecutive elements at any distance: as it is, or copied.
 Tensor rows_of(const Tensor& t) {
+    if (t.is_neg()) return t.resolve_neg().contiguous();
     const bool ok = t.stride(-1) == 1 || t.size(-1) <= 1;
     return ok && (t.dim() < 2 || t.stride(-2) >= 0) ? t : t.contiguous();
 }
@@ -89,6 +94,7 @@ void expect_out(const Tensor& t, const char* name, at::ScalarType type, at::IntA
     expect_type(t, name, type);
     expect_shape(t, name, shape);
     expect_device(t, name, like);
+    TORCH_CHECK_VALUE(!t.is_neg(), name, " must not be a negated view");
     TORCH_CHECK_VALUE(t.numel() == 0 || t.dim() != 2 ||
                           ((t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))),
                       name, " must have rows of consecutive elements that do not overlap, got strides ", t.strides());
@@ -276,7 +282,7 @@ struct UnpermuteFn : torch::autograd::Function<UnpermuteFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& offsets, const Tensor& row_of_slot,
                           const OptTensor& weights) {
         const Plan p = plan_of(offsets, row_of_slot, rows);
-        const Tensor w = weights ? weights->contiguous() : Tensor();
+        const Tensor w = weights ? dense(*weights) : Tensor();
         // rows are read again for the gradient of the weights alone
         const bool keep = weights && weights->requires_grad();
         ctx->save_for_backward({p.offsets, p.row_of_slot, w, keep ? rows : Tensor()});
@@ -329,14 +335,14 @@ Tensor unpermute(const Tensor& rows, const Tensor& offsets, const Tensor& row_of
         written(*out);
         if (out->numel() == 0) return *out;
         On on(rows);
-        const Tensor in = rows_of(rows), wc = w.defined() ? w.contiguous() : w;
+        const Tensor in = rows_of(rows), wc = w.defined() ? dense(w) : w;
         check(mi_experts_unpermute(dtype, in.const_data_ptr(), row_stride(in), p.T, (int32_t)p.k, in.size(1), p.rows(),
                                    p.count(), wc.defined() ? wc.const_data_ptr<float>() : nullptr,
                                    out->mutable_data_ptr(), row_stride(*out), on.stream));
         return *out;
     }
     if (needs) return UnpermuteFn::apply(rows, p.offsets, p.row_of_slot, w.defined() ? OptTensor(w) : std::nullopt);
-    return unpermute_new(rows, p, w.defined() ? w.contiguous() : w);
+    return unpermute_new(rows, p, w.defined() ? dense(w) : w);
 }
 
 // The integer operators have no gradient: one that would be lost is refused.
@@ -466,14 +472,14 @@ Tensor int8_call(const Tensor& a, const Tensor& a_scale, const Tensor& b, const 
     const auto opt = a.options().requires_grad(false).dtype(out_type);
     Tensor out = given ? *out_opt : at::empty({rows, N}, opt);
     if (out.numel() == 0) return out;
-    const Tensor ac = rows_of(a), as = a_scale.contiguous(), bs = b_scale.contiguous();
+    const Tensor ac = rows_of(a), as = dense(a_scale), bs = dense(b_scale);
     const Tensor bc = rows_of(b);
     c.a = ac.const_data_ptr<int8_t>();
     c.a_scale = as.const_data_ptr<float>();
     c.b = bc.const_data_ptr<int8_t>();
     c.b_scale = bs.const_data_ptr<float>();
     if (bias && bias->defined()) {
-        bias_c = bias->contiguous();
+        bias_c = dense(*bias);
         c.bias = bias_c.const_data_ptr();
         c.bias_dtype = out_dtype_of(bias_c.scalar_type());
     }

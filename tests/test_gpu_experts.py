@@ -391,3 +391,28 @@ def test_gradients_with_tangents_are_refused():
             with pytest.raises(ValueError, match="forward-mode"):
                 fa.permute(fwd.make_dual(x, torch.ones_like(x)), plan)
         assert all(bool((t == 2 if t is x else t >= 1).all()) for t in torch.autograd.grad(y, leaves, g))
+
+
+def test_negated_views():
+    """The imaginary part of a conjugate is a view whose sign is changed only when it is read; so may a gradient be."""
+    plan = fa.sort_experts(ids_of(5, 2, 4, 1).cuda(), 4)
+    row = plan.token_of_row.long()
+    for H in (1, 24):
+        z = torch.complex(_rand((5, H), torch.float32, 1), _rand((5, H), torch.float32, 2)).conj()
+        x = z.imag
+        assert x.is_neg() and torch.equal(fa.permute(x, plan), x.resolve_neg()[row])
+        rows, w = fa.permute(x.resolve_neg(), plan), torch.complex(torch.ones(5, 2), torch.full((5, 2), 0.5)).cuda().conj().imag
+        y = fa.unpermute(rows, plan, w)
+        assert torch.equal(y, -fa.unpermute(rows, plan, -w.resolve_neg())) and torch.equal(y, -x.resolve_neg())
+        out = torch.zeros(10, H, dtype=torch.complex64, device="cuda").conj().imag
+        with pytest.raises(ValueError, match="negated"):
+            fa.permute(x, plan, out=out)
+        leaf = x.resolve_neg().clone().requires_grad_()
+        g = torch.ones(10, H, dtype=torch.complex64, device="cuda").mul_(1j).conj().imag  # -1
+        assert g.is_neg() and bool((torch.autograd.grad(fa.permute(leaf, plan), leaf, g)[0] == -2).all())
+    one = torch.ones(1, dtype=torch.complex64, device="cuda").mul_(2j).conj().imag  # -2, contiguous
+    assert one.is_neg() and one.is_contiguous()
+    plan = fa.sort_experts(torch.zeros(1, 1, dtype=torch.int32, device="cuda"), 1)
+    rows = torch.ones(1, 8, device="cuda", requires_grad=True)
+    y = fa.unpermute(rows, plan, one.view(1, 1))
+    assert bool((y == -2).all()) and bool((torch.autograd.grad(y.sum(), rows)[0] == -2).all())

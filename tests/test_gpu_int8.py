@@ -500,3 +500,25 @@ def test_refusals():
     assert fa.int8_grouped_matmul(a[:0], sa[:0], w, sw, offs * 0).shape == (0, 8)
     q, s = fa.quantize_int8(x[:0])
     assert q.shape == (0, 32) and s.shape == (0,)
+
+
+def test_negated_views():
+    """The imaginary part of a conjugate is a view whose sign is changed only when it is read."""
+    def neg(v, shape):
+        t = torch.full(shape, v * 1j, dtype=torch.complex64, device="cuda").conj().imag  # -v
+        assert t.is_neg()
+        return t
+
+    q, s = fa.quantize_int8(neg(3.0, (4, 1)))
+    assert bool((q == -127).all())
+    a, b = torch.ones(1, 16, dtype=torch.int8, device="cuda"), torch.ones(1, 16, dtype=torch.int8, device="cuda")
+    two, one = neg(2.0, (1,)), torch.ones(1, device="cuda")
+    assert two.is_contiguous()
+    f32 = torch.float32
+    assert float(fa.int8_matmul(a, two, b, one, out_dtype=f32)) == -32
+    assert float(fa.int8_matmul(a, one, b, two, out_dtype=f32)) == -32
+    assert float(fa.int8_matmul(a, one, b, one, bias=two, out_dtype=f32)) == 14
+    offs = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    assert float(fa.int8_grouped_matmul(a, two, b[None], two[None], offs, out_dtype=f32)) == 64
+    with pytest.raises(ValueError, match="negated"):
+        fa.int8_matmul(a, one, b, one, out=neg(0.0, (1, 1)))
