@@ -42,12 +42,26 @@ Int8Tile pick_tile(const Int8Call& p, bool wide) {
     return Int8Tile::T256x256;
 }
 
+// Whether a launch of this tile (a workgroup each, but for the 256 x 256 ones;
+// forms as in launch_int8_tile)
+// holds fewer than 2^32 threads. Calls are bounded by their 64 x 64 tiles, which
+// is enough for what pick_tile takes: smaller ones only for a few hundred.
+bool launch_fits(const Int8Call& p, Int8Tile tile) {
+    static const struct { int bm, bn, threads; } form[] = {
+        {32, 32, 1024}, {32, 64, 1024}, {64, 64, 512}, {64, 64, 256}, {64, 128, 512}, {64, 128, 256},
+        {128, 128, 512}, {128, 128, 256}};
+    if (tile == Int8Tile::T256x256) return true;
+    const auto& f = form[(int)tile];
+    return max_tiles(p.rows, f.bm, p.E) * ((p.N + f.bn - 1) / f.bn) * f.threads < (int64_t)1 << 32;
+}
+
 // MI_INT8_TILE = 0 .. 8 (an Int8Tile) takes that tile where a call can have it, for tests and timing.
-Int8Tile forced_tile(bool wide, Int8Tile tile) {
+Int8Tile forced_tile(const Int8Call& p, bool wide, Int8Tile tile) {
     const char* env = getenv("MI_INT8_TILE");
     if (!env || !*env) return tile;
     const int v = atoi(env);
-    return v >= 0 && v <= (int)Int8Tile::T256x256 - !wide ? (Int8Tile)v : tile;
+    if (v < 0 || v > (int)Int8Tile::T256x256 - !wide) return tile;
+    return launch_fits(p, (Int8Tile)v) ? (Int8Tile)v : tile;
 }
 
 // Dense products whose rows are no multiples of 16 bytes are copied to rows
@@ -100,7 +114,7 @@ hipError_t launch_int8_matmul(const mi_experts_int8_args& a, hipStream_t s) {
     const bool vec = (uint64_t)a.out % quad == 0 && a.out_stride % 4 == 0;
     const bool fast = bits % 16 == 0 && p.K % 16 == 0 && int8_offsets_fit(p, 256, 256);
     const bool wide = fast && p.K > 128;  // the 256 x 256 kernel takes two steps of 128 bytes at least
-    const Int8Tile tile = forced_tile(wide, pick_tile(p, wide));
+    const Int8Tile tile = forced_tile(p, wide, pick_tile(p, wide));
     if (tile == Int8Tile::T256x256) return launch_int8_wide(p, a.out_dtype, s);
     if (fast) return launch_int8_tile(p, a.out_dtype, tile, vec, s);
     return launch_int8_any(p, a.out_dtype, tile, vec, s);

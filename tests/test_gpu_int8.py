@@ -431,6 +431,17 @@ def test_expert_layer_in_int8(T):
         assert torch.equal(z, layer()[-1])
 
 
+@pytest.mark.parametrize("tile", [0, 1, 2])
+def test_forced_tiles_of_a_large_product(tile, monkeypatch):
+    """2^32 outputs: 32 x 32 tiles of 1024 threads would be 2^32 threads, the rule's tile is taken."""
+    n, K = 65536, 16
+    a, b, sa, sb = _ints((n, K), 1), _ints((n, K), 2), _scales(n, 3), _scales(n, 4)
+    monkeypatch.setenv("MI_INT8_TILE", str(tile))
+    y = fa.int8_matmul(a, sa, b, sb)
+    for rows in (slice(0, 40), slice(n // 2, n // 2 + 40), slice(n - 40, n)):
+        _check(y[rows], _exact(a[rows], b), sa[rows], sb)
+
+
 def test_two_streams_and_threads():
     import threading
     a, b, sa, sb = _ints((200, 2048), 1), _ints((1024, 2048), 2), _scales(200, 3), _scales(1024, 4)
