@@ -109,6 +109,31 @@ std::pair<const char*, const char*> extent(const Tensor& t) {
     return {p, p + (last + 1) * (int64_t)t.element_size()};
 }
 
+// Rows of `width` bytes, `pitch` apart; a vector at a distance is a column.
+struct Rows {
+    const char* first;
+    int64_t width, pitch, rows;
+};
+std::optional<Rows> as_rows(const Tensor& t) {
+    if (t.dim() < 1 || t.dim() > 2) return std::nullopt;
+    const bool column = t.dim() == 1 && t.stride(0) != 1;
+    if (t.dim() == 2 && t.size(1) > 1 && t.stride(1) != 1) return std::nullopt;
+    const int64_t size = (int64_t)t.element_size();
+    return Rows{static_cast<const char*>(t.const_data_ptr()), (column ? 1 : t.size(-1)) * size, t.stride(0) * size,
+                t.dim() == 2 || column ? t.size(0) : 1};
+}
+
+// Whether two tensors whose extents overlap are columns of one buffer that lie
+// side by side.
+bool side_by_side(const Tensor& x, const Tensor& y) {
+    auto a = as_rows(x), b = as_rows(y);
+    if (!a || !b) return false;
+    if (a->rows == 1) std::swap(a, b);  // one row lies beside rows of any pitch
+    if (a->pitch <= 0 || (b->rows > 1 && b->pitch != a->pitch)) return false;
+    const int64_t at = ((b->first - a->first) % a->pitch + a->pitch) % a->pitch;
+    return at >= a->width && at + b->width <= a->pitch;
+}
+
 // A destination shares no memory with what is read: rows are written while
 // others are read. Columns of one buffer may be both.
 void expect_apart(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
@@ -118,15 +143,7 @@ void expect_apart(const Tensor& out, const char* name, std::initializer_list<con
         if (!t->defined() || t->numel() == 0) continue;
         const auto i = extent(*t);
         if (i.second <= o.first || o.second <= i.first) continue;
-        if (t->dim() == 2 && out.dim() == 2 && t->size(0) > 1 && out.size(0) > 1) {
-            const int64_t pitch = out.stride(0) * (int64_t)out.element_size();
-            if (pitch > 0 && t->stride(0) * (int64_t)t->element_size() == pitch && t->stride(1) == 1) {
-                const int64_t w = t->size(1) * (int64_t)t->element_size(), n = out.size(1) * (int64_t)out.element_size();
-                const int64_t at = ((i.first - o.first) % pitch + pitch) % pitch;
-                if (at >= n && at + w <= pitch) continue;
-            }
-        }
-        TORCH_CHECK_VALUE(false, name, " shares memory with a tensor that the call reads");
+        TORCH_CHECK_VALUE(side_by_side(out, *t), name, " shares memory with a tensor that the call reads");
     }
 }
 

@@ -416,3 +416,33 @@ def test_negated_views():
     rows = torch.ones(1, 8, device="cuda", requires_grad=True)
     y = fa.unpermute(rows, plan, one.view(1, 1))
     assert bool((y == -2).all()) and bool((torch.autograd.grad(y.sum(), rows)[0] == -2).all())
+
+
+def test_columns_of_one_buffer():
+    """What a call reads and writes may lie side by side in one buffer, single rows and vectors too."""
+    H = 32
+    for T, k in ((1, 4), (3, 4), (4, 1), (1, 1)):
+        plan = fa.sort_experts(ids_of(T, k, 4, T).cuda(), 4)
+        n = T * k
+        x, rows, w = _rand((T, H), torch.float32, 1), _rand((n, H), torch.float32, 2), _rand((T, k), torch.float32, 3)
+        buf = torch.zeros(max(n, T * k), 2 * H + k, device="cuda")
+        buf[:T, H:2 * H] = x
+        assert torch.equal(fa.permute(buf[:T, H:2 * H], plan, out=buf[:n, :H]), fa.permute(x, plan))
+        buf[:n, H:2 * H], buf[:T, 2 * H:] = rows, w
+        y = fa.unpermute(buf[:n, H:2 * H], plan, buf[:T, 2 * H:], out=buf[:T, :H])
+        assert torch.equal(y, fa.unpermute(rows, plan, w))
+        if n > 1:
+            for lo in (0, 1, H - 1):
+                with pytest.raises(ValueError, match="shares memory"):
+                    fa.permute(buf[:T, lo:lo + H], plan, out=buf[:n, :H])
+                with pytest.raises(ValueError, match="shares memory"):
+                    fa.unpermute(buf[:n, :H], plan, out=buf[:T, lo:lo + H])
+            with pytest.raises(ValueError, match="shares memory"):  # into the next row
+                fa.permute(buf.view(-1)[2 * H + k - 1:][:H].view(1, H).expand(T, H), plan, out=buf[:n, :H])
+    # a column of scales beside the rows
+    q = torch.ones(6, 16, dtype=torch.int8, device="cuda")
+    buf = torch.full((6, 17), 0.5, device="cuda")
+    out = fa.int8_matmul(q, buf[:, 16], q[:1].expand(16, 16), torch.ones(16, device="cuda"), out=buf[:, :16])
+    assert bool((out == 8).all())
+    with pytest.raises(ValueError, match="shares memory"):
+        fa.int8_matmul(q, buf[:, 15], q[:1].expand(16, 16), torch.ones(16, device="cuda"), out=buf[:, :16])
