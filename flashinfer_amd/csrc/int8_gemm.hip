@@ -10,8 +10,10 @@
 
 namespace miexp {
 
+// A lane's offset: that of its row and a chunk inside 128 bytes. (Rows may
+// overlap, so the chunk is not inside the row's own distance.)
 bool int8_offsets_fit(const Int8Call& p, int bm, int bn) {
-    const int64_t most = (int64_t)1 << 32;
+    const int64_t most = ((int64_t)1 << 32) - 128;
     return (p.row_ids ? p.a_rows : (int64_t)bm) * p.a_stride < most && bn * p.b_stride < most;
 }
 

@@ -324,6 +324,21 @@ def test_gathered_rows_past_32_bits():
         _check(y[rows], _exact(a[ids[rows].long()], b[e]), sa[ids[rows].long()], sb[e])
 
 
+def test_gathered_overlapping_rows_at_32_bits():
+    """Rows that overlap (16 bytes apart, 128 long): the last ones' ends lie past 2^32 bytes, their starts before."""
+    M, K, N = 2 ** 28 - 1, 128, 64
+    line = torch.zeros((M - 1) * 16 + K, dtype=torch.int8, device="cuda")
+    line[:4096], line[-4096:] = _ints(4096, 1), _ints(4096, 2)
+    a = line.as_strided((M, K), (16, 1))
+    b, sb = _ints((2, N, K), 3), _scales((2, N), 4)
+    sa = torch.ones(M, device="cuda")
+    ids = torch.cat([torch.arange(M - 40, M), torch.arange(10)]).to(torch.int32).cuda()
+    offs = torch.tensor([0, 30, 50], dtype=torch.int32, device="cuda")
+    y = fa.int8_grouped_matmul(a, sa, b, sb, offs, row_ids=ids)
+    for e, rows in enumerate((slice(0, 30), slice(30, 50))):
+        _check(y[rows], _exact(a[ids[rows].long()], b[e]), sa[ids[rows].long()], sb[e])
+
+
 def test_copied_product_in_graphs():
     """Large products of rows at any address copy them to a workspace: two
     captured graphs, replayed in turn, keep theirs apart."""
