@@ -203,6 +203,30 @@ def test_every_tile(tile, shape, monkeypatch):
                 _check(y[at], _exact(a[src], b[e]), sa[src], sb[e])
 
 
+# few, some and many rows after each other, in all orders: at most 128, 129 to 192, up to 256, several tiles
+MIXED = [100, 300, 1, 0, 190, 256, 64, 64, 520, 128, 129, 700, 33, 256, 256, 140, 90, 150, 600, 300, 5, 130] * 2
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("K", [144, 256, 400, 640, 1040])  # 2, 2, 4, 5 and 9 steps; the last of 16 or 128 bytes
+def test_large_tiles_of_experts_in_turn(K, gather, monkeypatch):
+    """Workgroups with several 256 x 256 tiles, whose experts and row counts change from one to the next."""
+    monkeypatch.setenv("MI_INT8_TILE", "8")
+    E, R, N, dtype = len(MIXED), sum(MIXED), 4088, torch.float32 if K == 640 else torch.bfloat16
+    tiles = sum((c + 255) // 256 for c in MIXED) * 16
+    assert tiles > 3 * 256
+    offs = torch.tensor([0] + MIXED).cumsum(0).to(torch.int32).cuda()
+    M = 1500 if gather else R
+    a, b, sa, sb = _ints((M, K), 1), _ints((E, N, K), 2), _scales(M, 3), _scales((E, N), 4)
+    ids = torch.randint(0, M, (R,), generator=_gen(5), device="cuda", dtype=torch.int32) if gather else None
+    y = fa.int8_grouped_matmul(a, sa, b, sb, offs, row_ids=ids, out_dtype=dtype)
+    lo = 0
+    for e, c in enumerate(MIXED):
+        src = ids[lo:lo + c].long() if gather else slice(lo, lo + c)
+        _check(y[lo:lo + c], _exact(a[src], b[e]), sa[src], sb[e])
+        lo += c
+
+
 @pytest.mark.parametrize("K", [512, 515])
 @pytest.mark.parametrize("rows", [30, 400])
 def test_grouped_strided_weights_and_bad_ids(rows, K):
@@ -473,6 +497,41 @@ def test_two_streams_and_threads():
         bad.extend(0 for y in got if not torch.equal(y, want[:len(y)]))
 
     threads = [threading.Thread(target=work) for _ in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
+def test_streams_and_threads_with_workspaces():
+    """Calls that take a workspace, and those that clear what they do not use, on three streams at once:
+    every result is that of its own inputs."""
+    import threading
+    M, N, K, E, k = 2048, 2112, 4111, 8, 4
+    b, sb, w, sw = _ints((N, K), 1), _scales(N, 2), _ints((E, 512, 256), 3), _scales((E, 512), 4)
+    sa = _scales(M, 5)
+
+    def step(ids, a, x):
+        plan = fa.sort_experts(ids, E, 2)
+        q, s = fa.quantize_int8(x, num_rows=plan.expert_offsets[-1:])
+        return (*plan, q, s, fa.int8_grouped_matmul(q, s, w, sw, plan.expert_offsets), fa.int8_matmul(a, sa, b, sb))
+
+    inputs, want = [], []
+    for n in range(3):
+        ids = torch.randint(0, E + 4, (1500, k), generator=_gen(n), device="cuda", dtype=torch.int32)
+        inputs.append((ids, _ints((M, K), 10 + n), torch.randn(1500 * k, 256, generator=_gen(20 + n), device="cuda").half()))
+        want.append(step(*inputs[-1]))
+    _check(want[0][-1], _exact(inputs[0][1], b), sa, sb)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(n):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            got = [step(*inputs[n]) for _ in range(10)]
+            st.synchronize()
+        bad.extend((n, i, j) for i, out in enumerate(got) for j in range(len(out)) if not torch.equal(out[j], want[n][j]))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(3)]
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
