@@ -15,7 +15,7 @@
 // sums the counts of the chunks before its own, which are in L2. What bounds
 // it is the latency of a few dependent passes, not its 12 bytes a slot: 8
 // slots 4.2 us, 2048 6.6, 4096 8.5 (9.1 in one workgroup), 8000 8.4 (21),
-// 65536 13.5, a million 47.
+// 65536 13.5, a million 47 (on another box 8000 9.8, 65536 14.0, a million 48).
 #include "experts_common.hpp"
 
 namespace miexp {
@@ -24,9 +24,12 @@ constexpr int64_t SMALL = 3000;
 constexpr int64_t MAX_CHUNKS = 256;
 
 // Slots of a chunk. Short chunks shorten a wave's walk, many chunks the sums
-// over them: 16 to 20 of 512 or 1024 slots (8000 slots: 8.4 us, 9.5 in four;
-// 16384: 9.6 in 16, 10.7 in 32), 32 to 64 of 2048 to 4096 (65536: 13.5 in 32,
-// 18.4 in 16; 524288: 38 in 64, 43 in 256, 60 in 32), beyond 64 of 8192 up to 256.
+// over them: up to 10240 slots 6 to 20 chunks of 512 (8000 slots: 8.4 us in 16,
+// 9.5 in four), up to 32768 11 to 32 of 1024 (16384: 9.6 in 16, 10.7 in 32), up
+// to 131072 17 to 64 of 2048 (65536: 13.5 in 32, 18.4 in 16), up to 262144 33 to
+// 64 of 4096, then of 8192 and more, at most 256 (524288: 38 in 64, 43 in 256,
+// 60 in 32). Where the length doubles the time hardly steps: 32768 and 32776
+// slots 12.1 and 12.3 us, 131072 and 131080 18.0 and 20.4.
 inline int64_t chunk_len(int64_t slots) {
     int64_t len = 512;
     while (len * (len < 1024 ? 20 : len < 2048 ? 32 : len < 8192 ? 64 : MAX_CHUNKS) < slots) len *= 2;

@@ -8,7 +8,10 @@
 // its end, shifted down; a row of fewer than 16 is put together byte by byte.
 // Costs against aligned rows: 16 x 4096 x 7169 15.2 us (K = 7168 8.5), 1000 x
 // 1000 x 1000 7.3 (K = 1008 6.6), 8192 x 4096 x 7169 414 (189), which is why
-// large products are copied first (int8_gemm.hip).
+// large dense products with such a K are copied first (int8_gemm.hip). Others
+// of any size come here as they are: those whose strides or addresses alone are
+// off (8192 x 4096 x 7168 with one operand a byte off: 332), grouped ones, and
+// gathers from 2^32 bytes and more.
 #include "int8_common.hpp"
 
 namespace miexp {

@@ -20,9 +20,15 @@ bool int8_offsets_fit(const Int8Call& p, int bm, int bn) {
 // The tile of a product. Tiles are taken as large as still give each CU one
 // (256 of them), and K is shared inside a workgroup where that is what is left
 // to share. Experts with more tiles than that take tiles that hold their rows,
-// so that their weights are read once: those are what bounds the call. (Rows
-// of an expert: as many as there are at most, on average.) wide: 256 x 256
-// tiles are there too.
+// so that their weights are read once: those are what bounds the call. wide:
+// 256 x 256 tiles are there too.
+// The rows of an expert are known on the device alone. The host takes the rows
+// of the result over all experts, which a shard fills in part: with 32 of 256
+// experts it takes tiles for eight times the rows (4096 x 7168, 8 slots a token,
+// by the rule and by the best tile: 400 tokens 192 / 144 us with 64 x 128, 1000
+// 199 / 154 with 64 x 128, 3000 216 / 186 with 128 x 128, 8192 310 / 302 with the
+// rule's; 64 125 / 124). Experts that cannot have a row count as well: 2 rows 28 /
+// 16 with 32 x 32, but 8 rows of one token 37 / 37.
 Int8Tile pick_tile(const Int8Call& p, bool wide) {
     const int64_t groups = p.offsets ? p.E : 1, rows = (p.rows + groups - 1) / groups;
     auto tiles = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
@@ -44,10 +50,10 @@ Int8Tile pick_tile(const Int8Call& p, bool wide) {
     return Int8Tile::T256x256;
 }
 
-// Whether a launch of this tile (a workgroup each, but for the 256 x 256 ones;
-// forms as in launch_int8_tile)
-// holds fewer than 2^32 threads. Calls are bounded by their 64 x 64 tiles, which
-// is enough for what pick_tile takes: smaller ones only for a few hundred.
+// Whether a launch of this tile (forms as in launch_int8_tile; of the 256 x 256
+// ones at most 256 workgroups run) holds fewer than 2^32 threads. Calls are
+// bounded by their 64 x 64 tiles, which is enough for what pick_tile takes:
+// smaller ones only for a few hundred.
 bool launch_fits(const Int8Call& p, Int8Tile tile) {
     static const struct { int bm, bn, threads; } form[] = {
         {32, 32, 1024}, {32, 64, 1024}, {64, 64, 512}, {64, 64, 256}, {64, 128, 512}, {64, 128, 256},
@@ -66,11 +72,12 @@ Int8Tile forced_tile(const Int8Call& p, bool wide, Int8Tile tile) {
     return launch_fits(p, (Int8Tile)v) ? (Int8Tile)v : tile;
 }
 
-// Dense products whose rows are no multiples of 16 bytes are copied to rows
-// that are where that is less than what the kernels for any address lose: from
-// 2^20 tiles x bytes of K on (8192 x 4096 x 7169 414 -> 237 us, 2048 x 4096 x
-// 7169 127 -> 110, 3000 x 4000 x 1030 level, 1500 x 4096 x 2050 33.9 against
-// 35.4). Bytes of the copies, 0 for none.
+// Dense products whose K is no multiple of 16 are copied to rows that are one
+// where that is less than what the kernels for any address lose: from 2^20 tiles
+// x bytes of K on (8192 x 4096 x 7169 414 -> 227 to 237 us, 2048 x 4096 x 7169
+// 127 -> 110, 3000 x 4000 x 1030 level, 1500 x 4096 x 2050 33.9 against 35.4).
+// Strides and addresses do not count: the size of the workspace goes by the
+// sizes alone. Bytes of the copies, 0 for none.
 size_t int8_workspace(int64_t rows, int64_t N, int64_t K, int E) {
     const int64_t tiles = (rows + 127) / 128 * ((N + 127) / 128);
     const int64_t bytes = (rows + N) * ((K + 15) / 16 * 16);

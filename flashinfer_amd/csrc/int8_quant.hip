@@ -12,7 +12,9 @@
 // lane stay in registers between the two passes; longer rows are read (and,
 // with SwiGLU, computed) again. Bound by HBM and, with SwiGLU, nearly as much
 // by its arithmetic: 8192 x 2048 from bf16 15.2 us (3.3 TB/s), after SwiGLU 22
-// (3.8 TB/s); 8192 x 7168 43 and 64 us (4.1, 4.6 TB/s); 130 x 2048 3.4 us.
+// (3.8 TB/s); 8192 x 7168 39 to 43 and 64 to 73 us (4.1 to 4.5, 4.0 to 4.6
+// TB/s); 130 x 2048 3.4 us. Rows that are no multiples of 16 bytes go by single
+// elements: 8192 x 7172 85 and 122 us.
 // Zeros for rows that are not in use are written here, too: two fills ahead of
 // it made 10.7 us of 5.8 with 64 of 512 rows of 7168 in use.
 #include "experts_common.hpp"

@@ -33,8 +33,9 @@
 // whole takes 204 us, it is 178 without the copies, 188 without the LDS reads
 // and 140 without the MFMAs, so what is left is in the slots' ends. Experts'
 // products with few rows each are bound as much by their weights: 8192 rows
-// over 32 experts of 7168 x 2048 180-215 us for 604 MB and 0.24 TOP, 173
-// without the copies, 177 without the MFMAs.
+// over 32 experts of 7168 x 2048, drawn evenly, 190-194 us for 604 MB and 0.24
+// TOP (159 with exactly 256 rows each, a tile of rows); on a box where it took
+// 207-224, 173 without the copies and 177 without the MFMAs.
 //
 // Measured and left out: four waves of 128 x 128 (a third fewer LDS reads, but
 // copies only half a step ahead: 245 us), phases by halves of K instead of rows

@@ -67,7 +67,7 @@ def permute(hidden: torch.Tensor, plan: ExpertPlan, out: torch.Tensor | None = N
     ``out`` they stay as they were (a shard that has few of the slots writes
     only those).
 
-    Any dtype of 1 to 8 bytes; bfloat16, float16 and float32 are
+    Any real dtype of 1 to 8 bytes; bfloat16, float16 and float32 are
     differentiable (without ``out``). The gradient of a token is the sum of the
     gradients of its local rows, in fp32 in slot order, rounded once."""
     return _mi_experts.permute(hidden, plan[0], plan[2], out)

@@ -48,7 +48,8 @@ def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     float16 or float32; that of ``out`` if one is passed), rounded once.
 
     Rows may lie at any distance; K, strides and addresses that are multiples
-    of 16 take the fast kernels."""
+    of 16 take the fast kernels, and large products of another K are copied to
+    such rows first."""
     return _mi_experts.int8_matmul(a, a_scale, b, b_scale, bias, out_dtype, out)
 
 
@@ -63,5 +64,6 @@ def int8_grouped_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor,
     Row m of the product is row m of ``a``, or with ``row_ids`` (int32 [R]) row
     ``row_ids[m]``: ``plan.token_of_row`` multiplies tokens without laying them
     out first. Result [R, N]. Rows that no expert has are zeros, or stay as
-    they were in ``out``. An id that is no row of ``a`` gives a row of NaN."""
+    they were in ``out`` (a shard that has few of the rows writes only those).
+    An id that is no row of ``a`` gives a row of NaN."""
     return _mi_experts.int8_grouped_matmul(a, a_scale, b, b_scale, expert_offsets, row_ids, out_dtype, out)

@@ -481,6 +481,35 @@ def test_forced_tiles_of_a_large_product(tile, monkeypatch):
         _check(y[rows], _exact(a[rows], b), sa[rows], sb)
 
 
+@pytest.mark.parametrize("T", [1, 700])
+def test_expert_layer_into_buffers(T):
+    """On a shard whose experts have a part of the rows: buffers passed in, whose other rows hold anything, give what
+    new results give, and those rows stay."""
+    H, I, E, off, k = 256, 128, 8, 16, 4
+    ids = torch.rand(T, 64, generator=_gen(T), device="cuda").argsort(1)[:, :k].to(torch.int32)
+    ids[0, 0] = off
+    x, w = torch.randn(T, H, generator=_gen(1), device="cuda").bfloat16(), torch.rand(T, k, generator=_gen(2), device="cuda")
+    w1, w2 = _ints((E, 2 * I, H), 3), _ints((E, H, I), 4)
+    s1, s2 = _scales((E, 2 * I), 5), _scales((E, H), 6)
+    nan = float("nan")
+    h = torch.full((T * k, 2 * I), nan, dtype=torch.bfloat16, device="cuda")
+    qb, sb = torch.full((T * k, I), 77, dtype=torch.int8, device="cuda"), torch.full((T * k,), nan, device="cuda")
+    y = torch.full((T * k, H), nan, dtype=torch.bfloat16, device="cuda")
+
+    def layer(h, qb, sb, y):
+        plan = fa.sort_experts(ids, E, off)
+        q, s = fa.quantize_int8(x)
+        g = fa.int8_grouped_matmul(q, s, w1, s1, plan.expert_offsets, row_ids=plan.token_of_row, out=h)
+        q, s = fa.swiglu_quantize_int8(g, num_rows=plan.expert_offsets[-1:], q=qb, scale=sb)
+        return plan, fa.unpermute(fa.int8_grouped_matmul(q, s, w2, s2, plan.expert_offsets, out=y), plan, w)
+
+    want = layer(None, None, None, None)[1]
+    plan, got = layer(h, qb, sb, y)
+    S = int(plan.expert_offsets[-1])
+    assert torch.equal(got, want) and bool(torch.isfinite(got).all()) and 0 < S < T * k
+    assert bool((qb[S:] == 77).all()) and all(bool(torch.isnan(t[S:]).all()) for t in (h, sb, y))
+
+
 def test_two_streams_and_threads():
     import threading
     a, b, sa, sb = _ints((200, 2048), 1), _ints((1024, 2048), 2), _scales(200, 3), _scales(1024, 4)
