@@ -135,6 +135,10 @@ def _rows_of_experts(case, g):
     return starts.to(torch.int32), (order // k).to(torch.int32)
 
 
+def _rows_in_use(case):
+    return max(1, case["T"] * case["share"] // 100)
+
+
 def _inputs(case, seed):
     g, dtype = _generator(seed), TYPES[case["dtype"]]
     T = case["T"]
@@ -166,7 +170,7 @@ def _inputs(case, seed):
         state["x"] = floats(T, 2 * H).requires_grad_(case["train"])
         state["rows"] = None
         if case["share"] < 100:
-            state["rows"] = torch.tensor([T * case["share"] // 100], dtype=torch.int32, device="cuda")
+            state["rows"] = torch.tensor([_rows_in_use(case)], dtype=torch.int32, device="cuda")
         state["seed"] = torch.randint(0, 1 << 62, (1,), generator=g, device="cuda")
         if case["train"]:
             state["grad"] = floats(T, H)
@@ -346,12 +350,12 @@ def work(case):
             moved += 2 * T * E * size
         return {"bytes": moved, "flops": T * E * (12 if case["train"] else 6)}
     if case["op"] == "swiglu":
-        rows, H = T * case["share"] // 100, case["H"]
+        rows, H = _rows_in_use(case), case["H"]
         moved = 3 * rows * H * size
         if case["train"]:
             # results that the call allocates are written whole
             moved += 5 * rows * H * size + 3 * (T - rows) * H * size
-        return {"bytes": max(size, moved), "flops": rows * H * (20 if case["train"] else 6)}
+        return {"bytes": moved, "flops": rows * H * (20 if case["train"] else 6)}
     H, N, E = case["H"], case["N"], case["E"]
     rows, experts = T, 1
     if E:
