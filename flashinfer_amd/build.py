@@ -2,10 +2,11 @@
 definition: H=7168, I=2048, 32 of 256 experts, 8 groups, top-4 groups,
 top-8), one libmi_moe_<tag>.so per further definition in
 shapes.DEFINITIONS, libmi_experts.so (the operators around the experts, for
-any sizes), and libmi_peaks.so (achievable-peak probes used by bench.py), for
-gfx950 with hipcc; and two extensions of host C++ against torch's headers,
-built with g++: _mi_moe_host, the native host path of kernel.run, and
-_mi_experts, the torch side of the expert operators.
+any sizes), libmi_layer.so (those inside a layer of a caller's own), and
+libmi_peaks.so (achievable-peak probes used by bench.py), for gfx950 with
+hipcc; and three extensions of host C++ against torch's headers, built with
+g++: _mi_moe_host, the native host path of kernel.run, and _mi_experts and
+_mi_layer, the torch sides of the operators.
 
 Usage: python -m flashinfer_amd.build [--jobs N] [--save-temps]
 The shared libraries land next to this file so they travel with the tree.
@@ -33,6 +34,8 @@ EXPERTS_LIB = os.path.join(HERE, "libmi_experts.so")
 EXPERTS_SOURCES = ["experts_sort.hip", "experts_move.hip", "int8_quant.hip", "int8_gemm.hip", "int8_any.hip",
                    "int8_tile.hip", "int8_wide.hip",
                    "experts_capi.hip"]
+LAYER_LIB = os.path.join(HERE, "libmi_layer.so")
+LAYER_SOURCES = ["balance.hip", "swiglu.hip", "int4_pack.hip", "int4_gemm.hip", "int4_row.hip", "layer_capi.hip"]
 PEAKS_LIB = os.path.join(HERE, "libmi_peaks.so")
 PEAKS_SOURCES = ["peaks.hip"]
 # Per-source flags: MFMA results in VGPRs rather than AGPRs.
@@ -99,6 +102,9 @@ HOST_LIB = os.path.join(HERE, "_mi_moe_host" + sysconfig.get_config_var("EXT_SUF
 EXPERTS_SRC = os.path.join(CSRC, "experts_bind.cpp")
 EXPERTS_EXT = os.path.join(HERE, "_mi_experts" + sysconfig.get_config_var("EXT_SUFFIX"))
 
+LAYER_SRC = os.path.join(CSRC, "layer_bind.cpp")
+LAYER_EXT = os.path.join(HERE, "_mi_layer" + sysconfig.get_config_var("EXT_SUFFIX"))
+
 
 def _build_extension(src: str, out: str, links) -> str:
     """A torch extension of host code only, so g++ builds it (against torch's
@@ -134,23 +140,29 @@ def build_experts_ext() -> str:
     return _build_extension(EXPERTS_SRC, EXPERTS_EXT, ["-L", HERE, "-l:" + os.path.basename(EXPERTS_LIB)])
 
 
+def build_layer_ext() -> str:
+    """_mi_layer: the torch side of the layer's operators, linked to libmi_layer.so."""
+    return _build_extension(LAYER_SRC, LAYER_EXT, ["-L", HERE, "-l:" + os.path.basename(LAYER_LIB)])
+
+
 def build(jobs: int = 8, extra=()) -> str:
     bad = [d for d in DEFINITIONS if not definition_supported(d)]
     if bad:
         raise ValueError(f"unsupported definitions (see shapes.py): {bad}")
     os.makedirs(BUILD, exist_ok=True)
-    jobs_list = ([(s, d) for d in DEFINITIONS for s in SOURCES] + [(s, None) for s in EXPERTS_SOURCES]
-                 + [(s, None) for s in PEAKS_SOURCES])
+    shared = [(EXPERTS_SOURCES, EXPERTS_LIB), (LAYER_SOURCES, LAYER_LIB), (PEAKS_SOURCES, PEAKS_LIB)]
+    jobs_list = [(s, d) for d in DEFINITIONS for s in SOURCES] + [(s, None) for srcs, _ in shared for s in srcs]
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         objs = list(ex.map(lambda j: _compile(j[0], list(extra), j[1]), jobs_list))
     n = len(SOURCES)
     for k, d in enumerate(DEFINITIONS):
         _link(objs[k * n:(k + 1) * n], os.path.join(HERE, lib_name_of(d)))
     rest = objs[len(DEFINITIONS) * n:]
-    _link(rest[:len(EXPERTS_SOURCES)], EXPERTS_LIB)
-    _link(rest[len(EXPERTS_SOURCES):], PEAKS_LIB)
-    with ThreadPoolExecutor(max_workers=2) as ex:
-        for done in [ex.submit(build_host), ex.submit(build_experts_ext)]:
+    for srcs, out in shared:
+        _link(rest[:len(srcs)], out)
+        rest = rest[len(srcs):]
+    with ThreadPoolExecutor(max_workers=3) as ex:
+        for done in [ex.submit(build_host), ex.submit(build_experts_ext), ex.submit(build_layer_ext)]:
             done.result()
     return LIB
 

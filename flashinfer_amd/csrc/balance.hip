@@ -1,0 +1,459 @@
+// The balance loss of a router and the slots of each expert (mi_layer_balance),
+// and the gradient of its logits.
+//
+//   P[t, :] = softmax(l) or sigma(l) / sum sigma(l),  Pbar_s = sum_t P / n_s
+//   loss = 1/S' sum_s sum_e f_se Pbar_se,  f_se = E c_se / (k n_s)
+//   dl_j = g P_j (w_j - sum_e P_e w_e) (times 1 - sigma_j for the sigmoids),
+//   w_e = f_se / (n_s S') = dloss / dP_e
+//
+// Tokens go in chunks, and a piece is what one sequence has of one chunk: piece
+// number s + chunk rises along the batch, so the sequence of a piece is found
+// by bisection over g(s) = s + first(s) / chunk, and there are at most S +
+// chunks of them, whatever the lengths. A workgroup sums the probabilities and
+// counts the slots of its piece; a second launch sums the pieces of each
+// sequence, a third the sequences where there are more than one. All sums are
+// in a fixed order; the only atomics count whole numbers.
+#include "layer_common.hpp"
+
+namespace miexp {
+
+struct BalanceCall {
+    const void* logits;
+    const int32_t* ids;
+    const int32_t* offsets;
+    const uint8_t* mask;
+    float* loss;
+    int32_t* counts;
+    float* weights;
+    float* part;        // [pieces, E] sums of P
+    int32_t* part_n;    // [pieces, E + 1] slots, and tokens that count
+    float* seq_loss;    // [S]
+    int32_t* some;      // [S] whether the sequence has a token that counts
+    int64_t T, S, stride;
+    int E, k, chunk, sigmoid;
+    int64_t pieces;
+};
+
+// First token of sequence s, and of s + 1 its end: clamped and non-decreasing
+// from one to the next.
+__device__ __forceinline__ int64_t bound(const BalanceCall& p, int64_t s) {
+    if (!p.offsets) return s ? p.T : 0;
+    return max((int64_t)0, min((int64_t)p.offsets[s], p.T));
+}
+
+// The sequence of token t: the last one that starts at or before it, if t is
+// inside; -1 for a token of none.
+__device__ __forceinline__ int64_t sequence_of(const BalanceCall& p, int64_t t) {
+    if (!p.offsets) return 0;
+    int64_t lo = 0, hi = p.S;  // bound(lo) <= t < bound(hi), if it is inside at all
+    if (t < bound(p, 0) || t >= bound(p, p.S)) return -1;
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (bound(p, mid) <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// A wave's TX lanes hold a token's logits: lane j of them V at a time from j V,
+// STEPS times. Rows end where E does: lanes past it hold -inf.
+template <class T, int V, int STEPS, int TX>
+struct Row {
+    float x[STEPS][V];
+
+    __device__ __forceinline__ static int at(int i) { return (i * TX + (threadIdx.x & (TX - 1))) * V; }
+
+    __device__ __forceinline__ void load_row(const T* row, int E) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            if (at(i) + V <= E) {
+                load<T, V>(row + at(i), x[i]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[i][v] = at(i) + v < E ? (float)row[at(i) + v] : -INFINITY;
+            }
+        }
+    }
+    template <class F>
+    __device__ __forceinline__ static float over_lanes(float a, F f) {
+#pragma unroll
+        for (int d = TX / 2; d >= 1; d >>= 1) a = f(a, __shfl_xor(a, d, TX));
+        return a;
+    }
+    __device__ __forceinline__ static float sum(float a) {
+        return over_lanes(a, [](float b, float c) { return b + c; });
+    }
+    __device__ __forceinline__ static float largest(float a) {
+        return over_lanes(a, [](float b, float c) { return fmaxf(b, c); });
+    }
+    // x becomes P; `slope` 1 for the softmax, 1 - sigma for the sigmoids.
+    template <bool SLOPE>
+    __device__ __forceinline__ void scores(bool sigmoid, float (&slope)[STEPS][V]) {
+        float total = 0.f;
+        if (sigmoid) {
+            float l[STEPS][V];
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    l[i][v] = x[i][v];
+                    const float e = expf(-x[i][v]);
+                    const float s = 1.f / (1.f + e);
+                    // 1 - sigma without cancellation
+                    if constexpr (SLOPE) slope[i][v] = e < INFINITY ? e * s : 1.f;
+                    x[i][v] = s;
+                    total += s;
+                }
+            // Scores so low that their sigmoids, e^l, leave fp32: their quotients are those of e^(l - top).
+            if (sum(total) < 1e-30f) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) top = fmaxf(top, l[i][v]);
+                top = largest(top);
+                if (top == -INFINITY) top = 0.f;
+                total = 0.f;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        x[i][v] = expf(l[i][v] - top);
+                        total += x[i][v];
+                    }
+            }
+        } else {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) top = fmaxf(top, x[i][v]);
+            top = largest(top);
+            if (top == -INFINITY) top = 0.f;  // a row of them: zeros, whatever they are divided by
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if constexpr (SLOPE) slope[i][v] = 1.f;
+                    x[i][v] = expf(x[i][v] - top);
+                    total += x[i][v];
+                }
+        }
+        total = sum(total);
+        const float r = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[i][v] *= r;
+    }
+};
+
+// Sums of one piece. LDS: sums [waves][E], counts [E + 1].
+template <class T, int V, int STEPS, int TX>
+__global__ __launch_bounds__(256) void balance_piece_kernel(BalanceCall p) {
+    extern __shared__ float smem[];
+    constexpr int PER = 64 / TX;  // tokens of a wave at a time
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float* sums = smem;
+    int* counts = reinterpret_cast<int*>(smem + 4 * p.E);
+    // the last s with s + first(s) / chunk <= piece
+    const int64_t piece = blockIdx.x;
+    int64_t s = 0, hi = p.S;
+    while (hi - s > 1) {
+        const int64_t mid = (s + hi) >> 1;
+        if (mid + bound(p, mid) / p.chunk <= piece) s = mid; else hi = mid;
+    }
+    const int64_t c = piece - s;
+    const int64_t a = max(bound(p, s), c * p.chunk), z = min(bound(p, s + 1), (c + 1) * p.chunk);
+    for (int i = threadIdx.x; i <= p.E; i += 256) counts[i] = 0;
+    __syncthreads();
+    typedef Row<T, V, STEPS, TX> R;
+    float acc[STEPS][V] = {};
+    int mine = 0;  // tokens that count
+    for (int64_t t0 = a + wave * PER; t0 < z; t0 += 4 * PER) {
+        const int64_t t = t0 + lane / TX;
+        const bool live = t < z && (!p.mask || p.mask[t]);
+        if (__ballot(live) == 0) continue;
+        R row;
+        float none[STEPS][V];
+        row.load_row((const T*)p.logits + (live ? t : t0) * p.stride, p.E);
+        row.template scores<false>(p.sigmoid, none);
+        if (!live) continue;
+        ++mine;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[i][v] += row.x[i][v];
+        for (int j = lane & (TX - 1); j < p.k; j += TX) {
+            const int id = p.ids[t * p.k + j];
+            if (id >= 0 && id < p.E) atomicAdd(&counts[id], 1);
+        }
+    }
+    // the wave's tokens side by side, then the waves
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int d = TX; d < 64; d <<= 1) acc[i][v] += __shfl_xor(acc[i][v], d);
+            const int e = R::at(i) + v;
+            if (lane < TX && e < p.E) sums[wave * p.E + e] = acc[i][v];
+        }
+    if ((lane & (TX - 1)) == 0 && mine) atomicAdd(&counts[p.E], mine);
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += 256)
+        p.part[piece * p.E + e] = (sums[e] + sums[p.E + e]) + (sums[2 * p.E + e] + sums[3 * p.E + e]);
+    for (int e = threadIdx.x; e <= p.E; e += 256) p.part_n[piece * (p.E + 1) + e] = counts[e];
+}
+
+// Sum over a workgroup of 1024 threads of one value each, in a fixed order.
+__device__ __forceinline__ float block_sum(float v, float* tmp) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float all = 0.f;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) all += tmp[w];
+    __syncthreads();
+    return all;
+}
+
+// Sums the pieces of sequence blockIdx.x: COLUMNS threads side by side take the
+// experts, 1024 / COLUMNS rows of them the pieces.
+template <int COLUMNS>
+__global__ __launch_bounds__(1024) void balance_sum_kernel(BalanceCall p) {
+    constexpr int ROWS = 1024 / COLUMNS;
+    __shared__ float sum[1024], tmp[16];
+    __shared__ int num[1024];
+    const int64_t s = blockIdx.x, a = bound(p, s), z = bound(p, s + 1);
+    const int64_t first = s + a / p.chunk, end = z > a ? s + (z - 1) / p.chunk + 1 : first;
+    const int col = threadIdx.x % COLUMNS, row = threadIdx.x / COLUMNS;
+    int n = 0;
+    for (int64_t i = first + threadIdx.x; i < end; i += 1024) n += p.part_n[i * (p.E + 1) + p.E];
+    num[threadIdx.x] = n;
+    __syncthreads();
+    for (int d = 512; d >= 1; d >>= 1) {
+        if (threadIdx.x < d) num[threadIdx.x] += num[threadIdx.x + d];
+        __syncthreads();
+    }
+    n = num[0];
+    __syncthreads();
+    const float share = n ? 1.f / (float)n : 0.f, unit = share * (float)p.E / (float)p.k;
+    float loss = 0.f;
+    for (int e0 = 0; e0 < p.E; e0 += COLUMNS) {
+        const int e = e0 + col;
+        float x = 0.f;
+        int c = 0;
+        if (e < p.E)
+            for (int64_t i = first + row; i < end; i += ROWS) {
+                x += p.part[i * p.E + e];
+                c += p.part_n[i * (p.E + 1) + e];
+            }
+        sum[threadIdx.x] = x;
+        num[threadIdx.x] = c;
+        __syncthreads();
+        if (row == 0 && e < p.E) {
+            for (int r = 1; r < ROWS; ++r) {
+                x += sum[r * COLUMNS + col];
+                c += num[r * COLUMNS + col];
+            }
+            const float w = (float)c * unit * share;
+            p.counts[s * p.E + e] = c;
+            p.weights[s * p.E + e] = w;
+            loss += w * x;
+        }
+        __syncthreads();
+    }
+    loss = block_sum(loss, tmp);
+    if (threadIdx.x) return;
+    if (p.S == 1) {
+        p.loss[0] = loss;
+    } else {
+        p.seq_loss[s] = loss;
+        p.some[s] = n > 0;
+    }
+}
+
+// The mean over the sequences that have a token, and its share in each weight.
+__global__ __launch_bounds__(1024) void balance_mean_kernel(BalanceCall p) {
+    __shared__ float tmp[16];
+    float loss = 0.f, some = 0.f;
+    for (int64_t s = threadIdx.x; s < p.S; s += 1024) {
+        loss += p.seq_loss[s];
+        some += (float)p.some[s];  // whole numbers, exact up to 2^24
+    }
+    some = block_sum(some, tmp);
+    const float share = some > 0.f ? 1.f / some : 0.f;
+    if (blockIdx.x == 0) {
+        loss = block_sum(loss, tmp) * share;
+        if (threadIdx.x == 0) p.loss[0] = loss;
+    }
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < p.S * p.E; i += (int64_t)gridDim.x * 1024)
+        p.weights[i] *= share;
+}
+
+template <class T, int V, int STEPS, int TX>
+__global__ __launch_bounds__(256) void balance_backward_kernel(BalanceCall p, const float* __restrict__ grad_loss,
+                                                               T* __restrict__ grad, int64_t grad_stride) {
+    constexpr int PER = 64 / TX;
+    const int lane = threadIdx.x & 63;
+    const float g = *grad_loss;
+    typedef Row<T, V, STEPS, TX> R;
+    for (int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * PER; t0 < p.T; t0 += (int64_t)gridDim.x * 4 * PER) {
+        const int64_t t = t0 + lane / TX, from = min(t, p.T - 1);
+        int64_t s = sequence_of(p, from);
+        if (p.mask && !p.mask[from]) s = -1;
+        R row;
+        float slope[STEPS][V], w[STEPS][V];
+        row.load_row((const T*)p.logits + from * p.stride, p.E);
+        const float* weights = p.weights + max(s, (int64_t)0) * p.E;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[i][v] = R::at(i) + v < p.E ? weights[R::at(i) + v] : 0.f;
+        row.template scores<true>(p.sigmoid, slope);
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) dot = fmaf(row.x[i][v], w[i][v], dot);
+        dot = R::sum(dot);
+        if (t >= p.T) continue;
+        T* to = grad + t * grad_stride;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            float d[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                d[v] = s < 0 ? 0.f : g * (row.x[i][v] * slope[i][v] * (w[i][v] - dot));
+            if (R::at(i) + V <= p.E) {
+                store<T, V>(to + R::at(i), d);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (R::at(i) + v < p.E) to[R::at(i) + v] = (T)d[v];
+            }
+        }
+    }
+}
+
+// Tokens of a chunk: short ones for latency, at most 512 chunks or so for the
+// second launch's sums.
+int balance_chunk(int64_t T) {
+    int64_t chunk = 16;
+    while (chunk * 512 < T) chunk *= 2;
+    return (int)chunk;
+}
+int64_t balance_pieces(int64_t T, int64_t S) {
+    const int chunk = balance_chunk(T);
+    return S + (T + chunk - 1) / chunk;
+}
+
+struct BalanceSpace {
+    size_t part, part_n, seq_loss, some, total;
+};
+BalanceSpace balance_space(int64_t T, int64_t S, int E) {
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t pieces = (size_t)balance_pieces(T, S);
+    BalanceSpace b;
+    b.part = 0;
+    b.part_n = up(b.part + pieces * E * 4);
+    b.seq_loss = up(b.part_n + pieces * (E + 1) * 4);
+    b.some = up(b.seq_loss + (size_t)S * 4);
+    b.total = up(b.some + (size_t)S * 4);
+    return b;
+}
+size_t balance_workspace(int64_t T, int64_t S, int E) { return balance_space(T, S, E).total; }
+
+BalanceCall balance_call(const mi_layer_balance_args& a) {
+    BalanceCall p{};
+    p.logits = a.logits;
+    p.ids = a.topk_ids;
+    p.offsets = a.seq_offsets;
+    p.mask = a.mask;
+    p.loss = a.loss;
+    p.counts = a.counts;
+    p.weights = a.weights;
+    p.T = a.num_tokens;
+    p.S = a.num_seqs;
+    p.stride = a.logits_stride;
+    p.E = a.num_experts;
+    p.k = a.top_k;
+    p.chunk = balance_chunk(a.num_tokens);
+    p.sigmoid = a.score == MI_LAYER_SCORE_SIGMOID;
+    p.pieces = balance_pieces(a.num_tokens, a.num_seqs);
+    return p;
+}
+
+// Calls f with the form of a row: V values of a lane at a time (16 bytes, where
+// the rows are aligned to that), STEPS of them, TX lanes.
+template <class T, class F>
+hipError_t by_row(int E, bool vec, F f) {
+    constexpr int W = 16 / (int)sizeof(T);
+    if (vec) {
+        if (E <= 8 * W) return f(IntC<W>{}, IntC<1>{}, IntC<8>{});
+        if (E <= 16 * W) return f(IntC<W>{}, IntC<1>{}, IntC<16>{});
+        if (E <= 32 * W) return f(IntC<W>{}, IntC<1>{}, IntC<32>{});
+        if (E <= 64 * W) return f(IntC<W>{}, IntC<1>{}, IntC<64>{});
+        return f(IntC<W>{}, IntC<1024 / (64 * W)>{}, IntC<64>{});
+    }
+    if (E <= 64) return f(IntC<1>{}, IntC<1>{}, IntC<64>{});
+    if (E <= 256) return f(IntC<1>{}, IntC<4>{}, IntC<64>{});
+    return f(IntC<1>{}, IntC<16>{}, IntC<64>{});
+}
+template <class F>
+hipError_t by_type(int dtype, F f) {
+    if (dtype == MI_LAYER_F32) return f(float{});
+    if (dtype == MI_LAYER_F16) return f(_Float16{});
+    return f(__bf16{});
+}
+template <class T>
+bool balance_vec(const mi_layer_balance_args& a) {
+    return (uint64_t)a.logits % 16 == 0 && a.logits_stride % (16 / (int)sizeof(T)) == 0;
+}
+
+hipError_t launch_balance(const mi_layer_balance_args& a, hipStream_t s) {
+    BalanceCall p = balance_call(a);
+    const BalanceSpace b = balance_space(a.num_tokens, a.num_seqs, a.num_experts);
+    uint8_t* ws = (uint8_t*)a.workspace;
+    p.part = (float*)(ws + b.part);
+    p.part_n = (int32_t*)(ws + b.part_n);
+    p.seq_loss = (float*)(ws + b.seq_loss);
+    p.some = (int32_t*)(ws + b.some);
+    hipError_t e = by_type(a.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        return by_row<T>(a.num_experts, balance_vec<T>(a), [&](auto v, auto steps, auto tx) {
+            hipLaunchKernelGGL((balance_piece_kernel<T, decltype(v)::value, decltype(steps)::value, decltype(tx)::value>),
+                               dim3((unsigned)p.pieces), dim3(256), (size_t)(5 * p.E + 1) * 4, s, p);
+            return hipGetLastError();
+        });
+    });
+    if (e != hipSuccess) return e;
+    if (p.E <= 64)
+        hipLaunchKernelGGL(balance_sum_kernel<64>, dim3((unsigned)p.S), dim3(1024), 0, s, p);
+    else
+        hipLaunchKernelGGL(balance_sum_kernel<256>, dim3((unsigned)p.S), dim3(1024), 0, s, p);
+    e = hipGetLastError();
+    if (e != hipSuccess || p.S == 1) return e;
+    const int64_t blocks = (p.S * p.E + 1023) / 1024;
+    hipLaunchKernelGGL(balance_mean_kernel, dim3((unsigned)(blocks < 256 ? blocks : 256)), dim3(1024), 0, s, p);
+    return hipGetLastError();
+}
+
+hipError_t launch_balance_backward(const mi_layer_balance_args& a, const float* grad_loss, void* grad,
+                                   int64_t grad_stride, hipStream_t s) {
+    const BalanceCall p = balance_call(a);
+    return by_type(a.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        const bool vec = balance_vec<T>(a) && (uint64_t)grad % 16 == 0 && grad_stride % (16 / (int)sizeof(T)) == 0;
+        return by_row<T>(a.num_experts, vec, [&](auto v, auto steps, auto tx) {
+            constexpr int TX = decltype(tx)::value;
+            const int64_t blocks = (p.T + 4 * (64 / TX) - 1) / (4 * (64 / TX));
+            hipLaunchKernelGGL((balance_backward_kernel<T, decltype(v)::value, decltype(steps)::value, TX>),
+                               dim3((unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS)), dim3(256), 0, s, p,
+                               grad_loss, (T*)grad, grad_stride);
+            return hipGetLastError();
+        });
+    });
+}
+
+}  // namespace miexp

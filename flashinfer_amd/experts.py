@@ -14,28 +14,33 @@ can be captured into a graph. There is no CPU path.
 """
 from __future__ import annotations
 
+import importlib
 from typing import NamedTuple
 
 import torch
 
 
 class _Extension:
-    """flashinfer_amd/_mi_experts, loaded at the first call: the package has to
-    import before it is built. Loud if it is missing, as there is no other
+    """An extension of this package, loaded at the first call: the package has
+    to import before it is built. Loud if it is missing, as there is no other
     implementation."""
+
+    def __init__(self, module: str, names):
+        self.__dict__.update(_module=module, _names=names)
 
     def __getattr__(self, name):
         try:
-            from . import _mi_experts as ext
+            ext = importlib.import_module("." + self._module, __package__)
         except ImportError as e:
-            raise RuntimeError("flashinfer_amd/_mi_experts is missing or does not load: build it with "
+            raise RuntimeError(f"flashinfer_amd/{self._module} is missing or does not load: build it with "
                                f"`python -m flashinfer_amd.build` ({e})") from e
-        for n in ("sort_experts", "permute", "unpermute", "quantize", "int8_matmul", "int8_grouped_matmul"):
+        for n in self._names:
             self.__dict__[n] = getattr(ext, n)
         return getattr(ext, name)
 
 
-_mi_experts = _Extension()
+_mi_experts = _Extension("_mi_experts", ("sort_experts", "permute", "unpermute", "quantize", "int8_matmul",
+                                         "int8_grouped_matmul"))
 
 
 class ExpertPlan(NamedTuple):
