@@ -35,7 +35,8 @@ EXPERTS_SOURCES = ["experts_sort.hip", "experts_move.hip", "int8_quant.hip", "in
                    "int8_tile.hip", "int8_wide.hip",
                    "experts_capi.hip"]
 LAYER_LIB = os.path.join(HERE, "libmi_layer.so")
-LAYER_SOURCES = ["balance.hip", "swiglu.hip", "int4_pack.hip", "int4_gemm.hip", "int4_row.hip", "layer_capi.hip"]
+LAYER_SOURCES = ["balance.hip", "swiglu.hip", "int4_pack.hip", "int4_gemm.hip", "int4_row.hip", "int4_tile.hip",
+                 "layer_capi.hip"]
 PEAKS_LIB = os.path.join(HERE, "libmi_peaks.so")
 PEAKS_SOURCES = ["peaks.hip"]
 # Per-source flags: MFMA results in VGPRs rather than AGPRs.

@@ -154,6 +154,8 @@ hipError_t by_int4_types(int x_dtype, int scale_dtype, int group, F f) {
     return scale_dtype == MI_LAYER_F32 ? steps(__bf16{}, float{}) : steps(__bf16{}, __bf16{});
 }
 
+enum class Int4Tile { Row, T32x64, T64x128, T128x128, T256x192 };
+hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);
 hipError_t launch_int4_row(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hipStream_t s);
 
 }  // namespace miexp

@@ -1,6 +1,8 @@
 // Which kernel takes a product with 4-bit weights (mi_layer_int4_matmul).
 //
 //   out[m, n] = sum_g scale[g, n] (sum_{k in g} x[m, k] q[n, k]) + bias[n]
+#include <stdlib.h>
+
 #include "int4_common.hpp"
 
 namespace miexp {
@@ -22,6 +24,42 @@ __global__ __launch_bounds__(256) void int4_copy_kernel(const uint16_t* __restri
                 if (i * 8 + v < K) w[v / 2] |= (uint32_t)x[row * stride + i * 8 + v] << (16 * (v & 1));
             *reinterpret_cast<v4u*>(to + row * ld + i * 8) = w;
         }
+}
+
+// Whether the 32-bit offsets of the tiled kernels reach all of a tile's rows
+// (of x's, if they are gathered) and an expert's scales.
+bool int4_offsets_fit(const Int4Call& p) {
+    const int64_t most = ((int64_t)1 << 32) - 512;
+    return (p.row_ids ? p.a_rows : (int64_t)256) * p.x_stride * 2 < most && p.scale_expert * 4 < most;
+}
+
+Int4Tile pick_tile(const Int4Call& p) {
+    const int64_t groups = p.offsets ? p.E : 1, rows = (p.rows + groups - 1) / groups;
+    if (rows <= 16) return Int4Tile::Row;
+    if (rows <= 32) return Int4Tile::T32x64;
+    if (rows <= 64) return Int4Tile::T64x128;
+    auto tiles = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+    if (tiles(64, 128) <= 256) return Int4Tile::T64x128;
+    if (tiles(128, 128) <= 256) return Int4Tile::T128x128;
+    return Int4Tile::T256x192;
+}
+
+// Whether a launch of this tile holds fewer than 2^32 threads.
+bool launch_fits(const Int4Call& p, Int4Tile tile) {
+    static const struct { int bm, bn, threads; } form[] = {{32, 64, 512}, {64, 128, 512}, {128, 128, 512}, {256, 192, 512}};
+    if (tile == Int4Tile::Row) return true;
+    const auto& f = form[(int)tile - 1];
+    return max_tiles(p.rows, f.bm, p.E) * ((p.N + f.bn - 1) / f.bn) * f.threads < (int64_t)1 << 32;
+}
+
+// MI_INT4_TILE = 0 .. 4 (an Int4Tile) takes that tile where a call can have it, for tests and timing.
+Int4Tile forced_tile(const Int4Call& p, Int4Tile tile) {
+    const char* env = getenv("MI_INT4_TILE");
+    if (env && *env) {
+        const int v = atoi(env);
+        if (v >= 0 && v <= (int)Int4Tile::T256x192) tile = (Int4Tile)v;
+    }
+    return launch_fits(p, tile) && int4_offsets_fit(p) ? tile : Int4Tile::Row;
 }
 
 hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
@@ -62,7 +100,9 @@ hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
     }
     const uint64_t quad = a.out_dtype == MI_LAYER_F32 ? 16 : 8;
     const bool vec = (uint64_t)a.out % quad == 0 && a.out_stride % 4 == 0;
-    return launch_int4_row(p, a.x_dtype, a.scale_dtype, vec, s);
+    const Int4Tile tile = forced_tile(p, pick_tile(p));
+    if (tile == Int4Tile::Row) return launch_int4_row(p, a.x_dtype, a.scale_dtype, vec, s);
+    return launch_int4_tile(p, a.x_dtype, a.scale_dtype, tile, vec, s);
 }
 
 }  // namespace miexp

@@ -99,6 +99,51 @@ def test_matmul(shape, dtype):
     _check(fa.int4_matmul(x, w, bias=bias, out_dtype=torch.float32), x, full, bias)
 
 
+TILES = range(5)
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_every_tile(tile, monkeypatch):
+    """Each kernel at sizes that are its own and at those that are not."""
+    monkeypatch.setenv("MI_INT4_TILE", str(tile))
+    for n, (M, N, K) in enumerate(((1, 1, 8), (16, 64, 128), (33, 200, 136), (70, 131, 1000), (300, 400, 776),
+                                   (513, 260, 2048), (256, 192, 4104))):
+        for group in (32, 64, 128, 512):
+            dtype = TYPES[n % 2]
+            for scale_type in (dtype, torch.float32):
+                q, x = _q((N, K), n), _whole((M, K), dtype, n + 1)
+                scale = _powers((N, -(-K // group)), scale_type, n + 2)
+                y = fa.int4_matmul(x, fa.pack_int4(q, scale, group), out_dtype=torch.float32)
+                assert torch.equal(y.to(F64), torch.matmul(x.to(F64), _dequant(q, scale, group).t())), (M, N, K, group)
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_every_tile_grouped(tile, monkeypatch):
+    """Tiles of experts that follow each other, gathered and not, some without rows; rows that no expert has."""
+    monkeypatch.setenv("MI_INT4_TILE", str(tile))
+    counts, N, K, spare = [300, 0, 17, 129, 256, 1], 200, 520, 30
+    R, used = sum(counts) + spare, sum(counts)
+    offs = torch.tensor([0] + counts).cumsum(0).to(torch.int32).cuda() + 5
+    q, scale = _q((6, N, K), 1), _powers((6, N, 9), torch.float16, 2)
+    w = fa.pack_int4(q, scale, 64)
+    x = _whole((R + 100, K), torch.float16, 3)
+    ids = torch.randint(0, R + 100, (R,), generator=_gen(4), device="cuda", dtype=torch.int32)
+    ids[:5], ids[40], ids[-25:] = -1, R + 100, -1
+    for rows, table in ((x[:R], None), (x, ids)):
+        torch.full((R, N), 9.0, device="cuda")  # a freed block that holds no zeros, for the result to get
+        y = fa.int4_grouped_matmul(rows, w, offs, row_ids=table, out_dtype=torch.float32)
+        ref = torch.zeros(R, N, dtype=F64, device="cuda")
+        src = rows if table is None else rows[table.clamp(0, R + 99).long()]
+        lo = 5
+        for e, c in enumerate(counts):
+            ref[lo:lo + c] = torch.matmul(src[lo:lo + c].to(F64), _dequant(q[e], scale[e], 64).t())
+            lo += c
+        if table is not None:
+            assert bool(y[40].isnan().all())
+            y[40] = ref[40] = 0
+        assert torch.equal(y.to(F64), ref) and lo == used + 5
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_every_weight_at_every_place(dtype):
     """One-hot rows read the weights back: all 16 values, each place of a tile, clamped ones too."""
