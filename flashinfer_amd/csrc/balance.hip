@@ -11,8 +11,9 @@
 // by bisection over g(s) = s + first(s) / chunk, and there are at most S +
 // chunks of them, whatever the lengths. A workgroup sums the probabilities and
 // counts the slots of its piece; a second launch sums the pieces of each
-// sequence, a third the sequences where there are more than one. All sums are
-// in a fixed order; the only atomics count whole numbers.
+// sequence, in columns of experts where there are many; a third the columns and
+// the sequences, where there are more than one. All sums are in a fixed order;
+// the only atomics count whole numbers.
 #include "layer_common.hpp"
 
 namespace miexp {
@@ -27,10 +28,11 @@ struct BalanceCall {
     float* weights;
     float* part;        // [pieces, E] sums of P
     int32_t* part_n;    // [pieces, E + 1] slots, and tokens that count
-    float* seq_loss;    // [S]
+    float* seq_loss;    // [S, columns]
     int32_t* some;      // [S] whether the sequence has a token that counts
     int64_t T, S, stride;
     int E, k, chunk, sigmoid;
+    int columns;        // workgroups of the second launch for a sequence
     int64_t pieces;
 };
 
@@ -54,6 +56,40 @@ __device__ __forceinline__ int64_t sequence_of(const BalanceCall& p, int64_t t) 
     return lo;
 }
 
+// v of the lane that a DPP control names, in every lane (all lanes are there).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// f over groups of TX lanes, the same bits in each of them: pairs within 4
+// lanes, mirrored halves of 8 and 16, rows of 16 exchanged.
+template <int TX, class F>
+__device__ __forceinline__ float over_lanes(float a, F f) {
+    a = f(a, dpp<0xb1>(a));   // quad_perm 1 0 3 2
+    a = f(a, dpp<0x4e>(a));   // quad_perm 2 3 0 1
+    a = f(a, dpp<0x141>(a));  // row_half_mirror
+    if constexpr (TX >= 16) a = f(a, dpp<0x140>(a));  // row_mirror
+    if constexpr (TX >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+        a = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+    if constexpr (TX >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+        a = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+    return a;
+}
+
+// e^a = 2^(hi + lo) with hi + lo = a log2(e) to twice the precision; past 87
+// (2^125.5) in the precision of hi alone, below 2^-126 zero.
+__device__ __forceinline__ float exp_of(float a) {
+    constexpr float L2E = 1.44269502f, L2E_LO = 1.92596299e-8f, LN2 = 0.693147182f;
+    const float hi = a * L2E, lo = fmaf(a, L2E_LO, fmaf(a, L2E, -hi));
+    const float x = __builtin_amdgcn_exp2f(hi);
+    return fabsf(a) < 87.f ? fmaf(x, lo * LN2, x) : x;
+}
+
 // A wave's TX lanes hold a token's logits: lane j of them V at a time from j V,
 // STEPS times. Rows end where E does: lanes past it hold -inf.
 template <class T, int V, int STEPS, int TX>
@@ -73,17 +109,11 @@ struct Row {
             }
         }
     }
-    template <class F>
-    __device__ __forceinline__ static float over_lanes(float a, F f) {
-#pragma unroll
-        for (int d = TX / 2; d >= 1; d >>= 1) a = f(a, __shfl_xor(a, d, TX));
-        return a;
-    }
     __device__ __forceinline__ static float sum(float a) {
-        return over_lanes(a, [](float b, float c) { return b + c; });
+        return over_lanes<TX>(a, [](float b, float c) { return b + c; });
     }
     __device__ __forceinline__ static float largest(float a) {
-        return over_lanes(a, [](float b, float c) { return fmaxf(b, c); });
+        return over_lanes<TX>(a, [](float b, float c) { return fmaxf(b, c); });
     }
     // x becomes P; `slope` 1 for the softmax, 1 - sigma for the sigmoids.
     template <bool SLOPE>
@@ -96,15 +126,18 @@ struct Row {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     l[i][v] = x[i][v];
-                    const float e = expf(-x[i][v]);
-                    const float s = 1.f / (1.f + e);
+                    const float e = exp_of(-x[i][v]);
+                    const float d = 1.f + e, rc = __builtin_amdgcn_rcpf(d);
+                    // past 2^126 the reciprocal is 0, and so is such a score beside a sum of 1e-8
+                    const bool near = d < 8e37f;
+                    const float s = near ? fmaf(fmaf(-rc, d, 1.f), rc, rc) : rc;
                     // 1 - sigma without cancellation
-                    if constexpr (SLOPE) slope[i][v] = e < INFINITY ? e * s : 1.f;
+                    if constexpr (SLOPE) slope[i][v] = near ? e * s : 1.f;
                     x[i][v] = s;
                     total += s;
                 }
-            // Scores so low that their sigmoids, e^l, leave fp32: their quotients are those of e^(l - top).
-            if (sum(total) < 1e-30f) {
+            // Scores so low that their sigmoids are e^l in fp32: quotients of e^(l - top), which stay in range.
+            if (sum(total) < 1e-8f) {
                 float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i)
@@ -117,7 +150,7 @@ struct Row {
                 for (int i = 0; i < STEPS; ++i)
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        x[i][v] = expf(l[i][v] - top);
+                        x[i][v] = exp_of(l[i][v] - top);
                         total += x[i][v];
                     }
             }
@@ -134,7 +167,7 @@ struct Row {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     if constexpr (SLOPE) slope[i][v] = 1.f;
-                    x[i][v] = expf(x[i][v] - top);
+                    x[i][v] = exp_of(x[i][v] - top);
                     total += x[i][v];
                 }
         }
@@ -167,25 +200,40 @@ __global__ __launch_bounds__(256) void balance_piece_kernel(BalanceCall p) {
     for (int i = threadIdx.x; i <= p.E; i += 256) counts[i] = 0;
     __syncthreads();
     typedef Row<T, V, STEPS, TX> R;
+    constexpr int U = 16 / (STEPS * V) > 4 ? 4 : 16 / (STEPS * V);  // tokens on their way
     float acc[STEPS][V] = {};
     int mine = 0;  // tokens that count
-    for (int64_t t0 = a + wave * PER; t0 < z; t0 += 4 * PER) {
-        const int64_t t = t0 + lane / TX;
-        const bool live = t < z && (!p.mask || p.mask[t]);
-        if (__ballot(live) == 0) continue;
-        R row;
-        float none[STEPS][V];
-        row.load_row((const T*)p.logits + (live ? t : t0) * p.stride, p.E);
-        row.template scores<false>(p.sigmoid, none);
-        if (!live) continue;
-        ++mine;
+    for (int64_t t0 = a + wave * PER; t0 < z; t0 += 4 * PER * U) {
+        R row[U];
+        bool live[U];
+        int id[U];
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i)
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t0 + u * 4 * PER + lane / TX;
+            live[u] = t < z && (!p.mask || p.mask[t]);
+            const int64_t from = live[u] ? t : t0;
+            row[u].load_row((const T*)p.logits + from * p.stride, p.E);
+            const int j = lane & (TX - 1);
+            id[u] = live[u] && j < p.k ? p.ids[from * p.k + j] : -1;
+        }
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc[i][v] += row.x[i][v];
-        for (int j = lane & (TX - 1); j < p.k; j += TX) {
-            const int id = p.ids[t * p.k + j];
-            if (id >= 0 && id < p.E) atomicAdd(&counts[id], 1);
+        for (int u = 0; u < U; ++u) {
+            float none[STEPS][V];
+            row[u].template scores<false>(p.sigmoid, none);
+            if (!live[u]) continue;
+            ++mine;
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[i][v] += row[u].x[i][v];
+            if (id[u] >= 0 && id[u] < p.E) atomicAdd(&counts[id[u]], 1);
+            if (TX < MI_LAYER_MAX_TOP_K && p.k > TX) {
+                const int64_t t = t0 + u * 4 * PER + lane / TX;
+                for (int j = (lane & (TX - 1)) + TX; j < p.k; j += TX) {
+                    const int e = p.ids[t * p.k + j];
+                    if (e >= 0 && e < p.E) atomicAdd(&counts[e], 1);
+                }
+            }
         }
     }
     // the wave's tokens side by side, then the waves
@@ -217,41 +265,46 @@ __device__ __forceinline__ float block_sum(float v, float* tmp) {
     return all;
 }
 
-// Sums the pieces of sequence blockIdx.x: COLUMNS threads side by side take the
-// experts, 1024 / COLUMNS rows of them the pieces.
+// Sums the pieces of sequence blockIdx.x / p.columns, of its columns of experts
+// (all of them in turn if p.columns is 1): COLUMNS threads side by side take
+// the experts, 1024 / COLUMNS rows of them the pieces.
 template <int COLUMNS>
 __global__ __launch_bounds__(1024) void balance_sum_kernel(BalanceCall p) {
     constexpr int ROWS = 1024 / COLUMNS;
     __shared__ float sum[1024], tmp[16];
     __shared__ int num[1024];
-    const int64_t s = blockIdx.x, a = bound(p, s), z = bound(p, s + 1);
+    const int64_t s = blockIdx.x / p.columns, a = bound(p, s), z = bound(p, s + 1);
+    const int part = (int)(blockIdx.x - s * p.columns);
     const int64_t first = s + a / p.chunk, end = z > a ? s + (z - 1) / p.chunk + 1 : first;
     const int col = threadIdx.x % COLUMNS, row = threadIdx.x / COLUMNS;
     int n = 0;
     for (int64_t i = first + threadIdx.x; i < end; i += 1024) n += p.part_n[i * (p.E + 1) + p.E];
-    num[threadIdx.x] = n;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d);
+    if ((threadIdx.x & 63) == 0) num[threadIdx.x >> 6] = n;
     __syncthreads();
-    for (int d = 512; d >= 1; d >>= 1) {
-        if (threadIdx.x < d) num[threadIdx.x] += num[threadIdx.x + d];
-        __syncthreads();
-    }
-    n = num[0];
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) n += num[w];
     __syncthreads();
     const float share = n ? 1.f / (float)n : 0.f, unit = share * (float)p.E / (float)p.k;
     float loss = 0.f;
-    for (int e0 = 0; e0 < p.E; e0 += COLUMNS) {
+    for (int e0 = part * COLUMNS; e0 < p.E; e0 += COLUMNS * p.columns) {
         const int e = e0 + col;
         float x = 0.f;
         int c = 0;
-        if (e < p.E)
+        if (e < p.E) {
+#pragma unroll 4
             for (int64_t i = first + row; i < end; i += ROWS) {
                 x += p.part[i * p.E + e];
                 c += p.part_n[i * (p.E + 1) + e];
             }
+        }
         sum[threadIdx.x] = x;
         num[threadIdx.x] = c;
         __syncthreads();
         if (row == 0 && e < p.E) {
+#pragma unroll 8
             for (int r = 1; r < ROWS; ++r) {
                 x += sum[r * COLUMNS + col];
                 c += num[r * COLUMNS + col];
@@ -265,11 +318,11 @@ __global__ __launch_bounds__(1024) void balance_sum_kernel(BalanceCall p) {
     }
     loss = block_sum(loss, tmp);
     if (threadIdx.x) return;
-    if (p.S == 1) {
+    if (p.S == 1 && p.columns == 1) {
         p.loss[0] = loss;
     } else {
-        p.seq_loss[s] = loss;
-        p.some[s] = n > 0;
+        p.seq_loss[blockIdx.x] = loss;
+        if (part == 0) p.some[s] = n > 0;
     }
 }
 
@@ -277,71 +330,91 @@ __global__ __launch_bounds__(1024) void balance_sum_kernel(BalanceCall p) {
 __global__ __launch_bounds__(1024) void balance_mean_kernel(BalanceCall p) {
     __shared__ float tmp[16];
     float loss = 0.f, some = 0.f;
-    for (int64_t s = threadIdx.x; s < p.S; s += 1024) {
-        loss += p.seq_loss[s];
-        some += (float)p.some[s];  // whole numbers, exact up to 2^24
-    }
+    for (int64_t i = threadIdx.x; i < p.S * p.columns; i += 1024) loss += p.seq_loss[i];
+    for (int64_t s = threadIdx.x; s < p.S; s += 1024) some += (float)p.some[s];  // whole numbers, exact up to 2^24
     some = block_sum(some, tmp);
     const float share = some > 0.f ? 1.f / some : 0.f;
     if (blockIdx.x == 0) {
         loss = block_sum(loss, tmp) * share;
         if (threadIdx.x == 0) p.loss[0] = loss;
     }
+    if (p.S == 1) return;
     for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < p.S * p.E; i += (int64_t)gridDim.x * 1024)
         p.weights[i] *= share;
 }
 
-template <class T, int V, int STEPS, int TX>
+// SEQS: tokens look up their sequence and its weights; else all have the same,
+// which stay in registers.
+template <class T, int V, int STEPS, int TX, bool SEQS>
 __global__ __launch_bounds__(256) void balance_backward_kernel(BalanceCall p, const float* __restrict__ grad_loss,
                                                                T* __restrict__ grad, int64_t grad_stride) {
-    constexpr int PER = 64 / TX;
+    constexpr int PER = 64 / TX, U = STEPS * V > 4 ? 1 : 2;  // tokens on their way
     const int lane = threadIdx.x & 63;
     const float g = *grad_loss;
     typedef Row<T, V, STEPS, TX> R;
-    for (int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * PER; t0 < p.T; t0 += (int64_t)gridDim.x * 4 * PER) {
-        const int64_t t = t0 + lane / TX, from = min(t, p.T - 1);
-        int64_t s = sequence_of(p, from);
-        if (p.mask && !p.mask[from]) s = -1;
-        R row;
-        float slope[STEPS][V], w[STEPS][V];
-        row.load_row((const T*)p.logits + from * p.stride, p.E);
-        const float* weights = p.weights + max(s, (int64_t)0) * p.E;
+    float w[STEPS][V];
+    auto weights_of = [&](int64_t s) __attribute__((always_inline)) {
+        const float* from = p.weights + s * p.E;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-            for (int v = 0; v < V; ++v) w[i][v] = R::at(i) + v < p.E ? weights[R::at(i) + v] : 0.f;
-        row.template scores<true>(p.sigmoid, slope);
-        float dot = 0.f;
+            for (int v = 0; v < V; ++v) w[i][v] = R::at(i) + v < p.E ? from[R::at(i) + v] : 0.f;
+    };
+    if constexpr (!SEQS) weights_of(0);
+    const int64_t step = (int64_t)gridDim.x * 4 * PER;
+    for (int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * PER; t0 < p.T; t0 += step * U) {
+        R row[U];
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i)
+        for (int u = 0; u < U; ++u)
+            row[u].load_row((const T*)p.logits + min(t0 + u * step + lane / TX, p.T - 1) * p.stride, p.E);
 #pragma unroll
-            for (int v = 0; v < V; ++v) dot = fmaf(row.x[i][v], w[i][v], dot);
-        dot = R::sum(dot);
-        if (t >= p.T) continue;
-        T* to = grad + t * grad_stride;
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = t0 + u * step + lane / TX, from = min(t, p.T - 1);
+            bool out = p.mask && !p.mask[from];
+            if constexpr (SEQS) {
+                const int64_t s = sequence_of(p, from);
+                weights_of(max(s, (int64_t)0));
+                out |= s < 0;
+            }
+            float slope[STEPS][V];
+            row[u].template scores<true>(p.sigmoid, slope);
+            float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            float d[V];
+            for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                d[v] = s < 0 ? 0.f : g * (row.x[i][v] * slope[i][v] * (w[i][v] - dot));
-            if (R::at(i) + V <= p.E) {
-                store<T, V>(to + R::at(i), d);
-            } else {
+                for (int v = 0; v < V; ++v) dot = fmaf(row[u].x[i][v], w[i][v], dot);
+            dot = R::sum(dot);
+            if (t >= p.T) continue;
+            T* to = grad + t * grad_stride;
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                float d[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (R::at(i) + v < p.E) to[R::at(i) + v] = (T)d[v];
+                    d[v] = out ? 0.f : g * (row[u].x[i][v] * slope[i][v] * (w[i][v] - dot));
+                if (R::at(i) + V <= p.E) {
+                    store<T, V>(to + R::at(i), d);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+                        if (R::at(i) + v < p.E) to[R::at(i) + v] = (T)d[v];
+                }
             }
         }
     }
 }
 
-// Tokens of a chunk: short ones for latency, at most 512 chunks or so for the
-// second launch's sums.
+// Tokens of a chunk: short ones for latency, then as many as keep the chunks at
+// 2048, eight workgroups for each CU.
 int balance_chunk(int64_t T) {
     int64_t chunk = 16;
-    while (chunk * 512 < T) chunk *= 2;
+    while (chunk * 2048 < T) chunk *= 2;
     return (int)chunk;
+}
+// Workgroups that sum a sequence's pieces: one, or where a few sequences have
+// many, one for 16 experts.
+int balance_columns(int64_t T, int64_t S, int E) {
+    return S <= 16 && T / balance_chunk(T) / S > 128 ? (E + 15) / 16 : 1;
 }
 int64_t balance_pieces(int64_t T, int64_t S) {
     const int chunk = balance_chunk(T);
@@ -358,7 +431,7 @@ BalanceSpace balance_space(int64_t T, int64_t S, int E) {
     b.part = 0;
     b.part_n = up(b.part + pieces * E * 4);
     b.seq_loss = up(b.part_n + pieces * (E + 1) * 4);
-    b.some = up(b.seq_loss + (size_t)S * 4);
+    b.some = up(b.seq_loss + (size_t)S * balance_columns(T, S, E) * 4);
     b.total = up(b.some + (size_t)S * 4);
     return b;
 }
@@ -379,6 +452,7 @@ BalanceCall balance_call(const mi_layer_balance_args& a) {
     p.E = a.num_experts;
     p.k = a.top_k;
     p.chunk = balance_chunk(a.num_tokens);
+    p.columns = balance_columns(a.num_tokens, a.num_seqs, a.num_experts);
     p.sigmoid = a.score == MI_LAYER_SCORE_SIGMOID;
     p.pieces = balance_pieces(a.num_tokens, a.num_seqs);
     return p;
@@ -428,13 +502,15 @@ hipError_t launch_balance(const mi_layer_balance_args& a, hipStream_t s) {
         });
     });
     if (e != hipSuccess) return e;
-    if (p.E <= 64)
+    if (p.columns > 1)
+        hipLaunchKernelGGL(balance_sum_kernel<16>, dim3((unsigned)(p.S * p.columns)), dim3(1024), 0, s, p);
+    else if (p.E <= 64)
         hipLaunchKernelGGL(balance_sum_kernel<64>, dim3((unsigned)p.S), dim3(1024), 0, s, p);
     else
         hipLaunchKernelGGL(balance_sum_kernel<256>, dim3((unsigned)p.S), dim3(1024), 0, s, p);
     e = hipGetLastError();
-    if (e != hipSuccess || p.S == 1) return e;
-    const int64_t blocks = (p.S * p.E + 1023) / 1024;
+    if (e != hipSuccess || (p.S == 1 && p.columns == 1)) return e;
+    const int64_t blocks = p.S == 1 ? 1 : (p.S * p.E + 1023) / 1024;
     hipLaunchKernelGGL(balance_mean_kernel, dim3((unsigned)(blocks < 256 ? blocks : 256)), dim3(1024), 0, s, p);
     return hipGetLastError();
 }
@@ -447,11 +523,16 @@ hipError_t launch_balance_backward(const mi_layer_balance_args& a, const float* 
         const bool vec = balance_vec<T>(a) && (uint64_t)grad % 16 == 0 && grad_stride % (16 / (int)sizeof(T)) == 0;
         return by_row<T>(a.num_experts, vec, [&](auto v, auto steps, auto tx) {
             constexpr int TX = decltype(tx)::value;
+            // 8 workgroups for each CU go over the tokens
             const int64_t blocks = (p.T + 4 * (64 / TX) - 1) / (4 * (64 / TX));
-            hipLaunchKernelGGL((balance_backward_kernel<T, decltype(v)::value, decltype(steps)::value, TX>),
-                               dim3((unsigned)(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS)), dim3(256), 0, s, p,
-                               grad_loss, (T*)grad, grad_stride);
-            return hipGetLastError();
+            const dim3 grid((unsigned)(blocks < 2048 ? blocks : 2048));
+            auto launch = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p, grad_loss, (T*)grad, grad_stride);
+                return hipGetLastError();
+            };
+            constexpr int VV = decltype(v)::value, ST = decltype(steps)::value;
+            return p.offsets ? launch(balance_backward_kernel<T, VV, ST, TX, true>)
+                             : launch(balance_backward_kernel<T, VV, ST, TX, false>);
         });
     });
 }

@@ -57,7 +57,8 @@ Int4Tile forced_tile(const Int4Call& p, Int4Tile tile) {
     const char* env = getenv("MI_INT4_TILE");
     if (env && *env) {
         const int v = atoi(env);
-        if (v >= 0 && v <= (int)Int4Tile::T256x192) tile = (Int4Tile)v;
+        if (v>4) return (Int4Tile)v;
+ if (v >= 0 && v <= (int)Int4Tile::T256x192) tile = (Int4Tile)v;
     }
     return launch_fits(p, tile) && int4_offsets_fit(p) ? tile : Int4Tile::Row;
 }

@@ -218,6 +218,12 @@ hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int
         case Int4Tile::T32x64: return launch<2, 1, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T64x128: return launch<4, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T128x128: return launch<4, 2, 2, 4, 3, 1>(p, x_dtype, scale_dtype, vec, s);
+        case (Int4Tile)5: return launch<1, 1, 1, 4, 4, 2>(p, x_dtype, scale_dtype, vec, s);
+        case (Int4Tile)6: return launch<1, 1, 1, 4, 4, 4>(p, x_dtype, scale_dtype, vec, s);
+        case (Int4Tile)7: return launch<1, 1, 1, 2, 5, 4>(p, x_dtype, scale_dtype, vec, s);
+        case (Int4Tile)8: return launch<1, 1, 1, 1, 3, 8>(p, x_dtype, scale_dtype, vec, s);
+        case (Int4Tile)9: return launch<1, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
+        case (Int4Tile)10: return launch<2, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
         default: return launch<8, 3, 2, 4, 2, 1>(p, x_dtype, scale_dtype, vec, s);
     }
 }
