@@ -180,14 +180,14 @@ struct Row {
     }
 };
 
-// Sums of one piece. LDS: sums [waves][E], counts [E + 1].
-template <class T, int V, int STEPS, int TX>
-__global__ __launch_bounds__(256) void balance_piece_kernel(BalanceCall p) {
+// Sums of one piece by WAVES waves. LDS: sums [min(WAVES, 8)][E], counts [E + 1].
+template <class T, int V, int STEPS, int TX, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void balance_piece_kernel(BalanceCall p) {
     extern __shared__ float smem[];
-    constexpr int PER = 64 / TX;  // tokens of a wave at a time
+    constexpr int PER = 64 / TX, HALF = WAVES > 8 ? 8 : WAVES;  // PER: tokens of a wave at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float* sums = smem;
-    int* counts = reinterpret_cast<int*>(smem + 4 * p.E);
+    int* counts = reinterpret_cast<int*>(smem + HALF * p.E);
     // the last s with s + first(s) / chunk <= piece
     const int64_t piece = blockIdx.x;
     int64_t s = 0, hi = p.S;
@@ -197,19 +197,19 @@ __global__ __launch_bounds__(256) void balance_piece_kernel(BalanceCall p) {
     }
     const int64_t c = piece - s;
     const int64_t a = max(bound(p, s), c * p.chunk), z = min(bound(p, s + 1), (c + 1) * p.chunk);
-    for (int i = threadIdx.x; i <= p.E; i += 256) counts[i] = 0;
+    for (int i = threadIdx.x; i <= p.E; i += 64 * WAVES) counts[i] = 0;
     __syncthreads();
     typedef Row<T, V, STEPS, TX> R;
     constexpr int U = 16 / (STEPS * V) > 4 ? 4 : 16 / (STEPS * V);  // tokens on their way
     float acc[STEPS][V] = {};
     int mine = 0;  // tokens that count
-    for (int64_t t0 = a + wave * PER; t0 < z; t0 += 4 * PER * U) {
+    for (int64_t t0 = a + wave * PER; t0 < z; t0 += WAVES * PER * U) {
         R row[U];
         bool live[U];
         int id[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t t = t0 + u * 4 * PER + lane / TX;
+            const int64_t t = t0 + u * WAVES * PER + lane / TX;
             live[u] = t < z && (!p.mask || p.mask[t]);
             const int64_t from = live[u] ? t : t0;
             row[u].load_row((const T*)p.logits + from * p.stride, p.E);
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256) void balance_piece_kernel(BalanceCall p) {
                 for (int v = 0; v < V; ++v) acc[i][v] += row[u].x[i][v];
             if (id[u] >= 0 && id[u] < p.E) atomicAdd(&counts[id[u]], 1);
             if (TX < MI_LAYER_MAX_TOP_K && p.k > TX) {
-                const int64_t t = t0 + u * 4 * PER + lane / TX;
+                const int64_t t = t0 + u * WAVES * PER + lane / TX;
                 for (int j = (lane & (TX - 1)) + TX; j < p.k; j += TX) {
                     const int e = p.ids[t * p.k + j];
                     if (e >= 0 && e < p.E) atomicAdd(&counts[e], 1);
@@ -236,21 +236,38 @@ __global__ __launch_bounds__(256) void balance_piece_kernel(BalanceCall p) {
             }
         }
     }
-    // the wave's tokens side by side, then the waves
+    // the wave's tokens side by side, then the waves: the last eight of 16 to the first ones
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
+        for (int v = 0; v < V; ++v)
 #pragma unroll
             for (int d = TX; d < 64; d <<= 1) acc[i][v] += __shfl_xor(acc[i][v], d);
-            const int e = R::at(i) + v;
-            if (lane < TX && e < p.E) sums[wave * p.E + e] = acc[i][v];
-        }
     if ((lane & (TX - 1)) == 0 && mine) atomicAdd(&counts[p.E], mine);
+    auto each = [&](bool mine, auto f) {
+        if (!mine || lane >= TX) return;
+        float* row = sums + (wave % HALF) * p.E;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (R::at(i) + v < p.E) f(row[R::at(i) + v], acc[i][v]);
+    };
+    if constexpr (WAVES > HALF) {
+        each(wave >= HALF, [](float& at, float& a) { at = a; });
+        __syncthreads();
+        each(wave < HALF, [](float& at, float& a) { at += a; });
+    } else {
+        each(true, [](float& at, float& a) { at = a; });
+    }
     __syncthreads();
-    for (int e = threadIdx.x; e < p.E; e += 256)
-        p.part[piece * p.E + e] = (sums[e] + sums[p.E + e]) + (sums[2 * p.E + e] + sums[3 * p.E + e]);
-    for (int e = threadIdx.x; e <= p.E; e += 256) p.part_n[piece * (p.E + 1) + e] = counts[e];
+    for (int e = threadIdx.x; e < p.E; e += 64 * WAVES) {
+        float all = 0.f;
+#pragma unroll
+        for (int w = 0; w < HALF; ++w) all += sums[w * p.E + e];
+        p.part[piece * p.E + e] = all;
+    }
+    for (int e = threadIdx.x; e <= p.E; e += 64 * WAVES) p.part_n[piece * (p.E + 1) + e] = counts[e];
 }
 
 // Sum over a workgroup of 1024 threads of one value each, in a fixed order.
@@ -404,17 +421,22 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(BalanceCall p, co
     }
 }
 
-// Tokens of a chunk: short ones for latency, then as many as keep the chunks at
-// 2048, eight workgroups for each CU.
+// Tokens of a chunk: 16 for four waves up to 4096 tokens, where latency counts;
+// then 64 or more for 16 waves, at most 512 chunks, two workgroups for each CU
+// (65536 x 256 in fp32: 18 us for the pieces and 21 for their sums with 2048
+// chunks of 32).
+constexpr int BALANCE_SHORT = 16;
 int balance_chunk(int64_t T) {
-    int64_t chunk = 16;
-    while (chunk * 2048 < T) chunk *= 2;
+    if (T <= 4096) return BALANCE_SHORT;
+    int64_t chunk = 64;
+    while (chunk * 512 < T) chunk *= 2;
     return (int)chunk;
 }
-// Workgroups that sum a sequence's pieces: one, or where a few sequences have
-// many, one for 16 experts.
+// Workgroups that sum a sequence's pieces: one, or one for 16 experts where that
+// takes off more than a launch that joins them (which several sequences need anyway).
 int balance_columns(int64_t T, int64_t S, int E) {
-    return S <= 16 && T / balance_chunk(T) / S > 128 ? (E + 15) / 16 : 1;
+    const int64_t pieces = T / balance_chunk(T) / S;
+    return pieces > (S > 1 ? 4 : 32) ? (E + 15) / 16 : 1;
 }
 int64_t balance_pieces(int64_t T, int64_t S) {
     const int chunk = balance_chunk(T);
@@ -496,8 +518,14 @@ hipError_t launch_balance(const mi_layer_balance_args& a, hipStream_t s) {
     hipError_t e = by_type(a.dtype, [&](auto t) {
         typedef decltype(t) T;
         return by_row<T>(a.num_experts, balance_vec<T>(a), [&](auto v, auto steps, auto tx) {
-            hipLaunchKernelGGL((balance_piece_kernel<T, decltype(v)::value, decltype(steps)::value, decltype(tx)::value>),
-                               dim3((unsigned)p.pieces), dim3(256), (size_t)(5 * p.E + 1) * 4, s, p);
+            constexpr int V = decltype(v)::value, STEPS = decltype(steps)::value, TX = decltype(tx)::value;
+            const dim3 grid((unsigned)p.pieces);
+            if (p.chunk == BALANCE_SHORT)
+                hipLaunchKernelGGL((balance_piece_kernel<T, V, STEPS, TX, 4>), grid, dim3(256),
+                                   (size_t)(5 * p.E + 1) * 4, s, p);
+            else
+                hipLaunchKernelGGL((balance_piece_kernel<T, V, STEPS, TX, 16>), grid, dim3(1024),
+                                   (size_t)(9 * p.E + 1) * 4, s, p);
             return hipGetLastError();
         });
     });
