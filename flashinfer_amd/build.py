@@ -36,7 +36,7 @@ EXPERTS_SOURCES = ["experts_sort.hip", "experts_move.hip", "int8_quant.hip", "in
                    "experts_capi.hip"]
 LAYER_LIB = os.path.join(HERE, "libmi_layer.so")
 LAYER_SOURCES = ["balance.hip", "swiglu.hip", "int4_pack.hip", "int4_gemm.hip", "int4_row.hip", "int4_tile.hip",
-                 "layer_capi.hip"]
+                 "int4_wide.hip", "layer_capi.hip"]
 PEAKS_LIB = os.path.join(HERE, "libmi_peaks.so")
 PEAKS_SOURCES = ["peaks.hip"]
 # Per-source flags: MFMA results in VGPRs rather than AGPRs.

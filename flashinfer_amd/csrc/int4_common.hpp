@@ -49,7 +49,7 @@ template <class XT> struct Operand;
 // upper half of that is it in bfloat16: 13 instructions for eight values.
 template <> struct Operand<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
-    static constexpr float UNIT = 16.f;  // a weight is in sixteenths
+    static constexpr float UNIT = 16.f;  // weights are made as sixteenths, and sums are multiplied at their end
     __device__ __forceinline__ static frag weights(uint32_t d) {
         const uint32_t h = d >> 4;
         float e[8];  // nibbles 0 .. 7
@@ -113,14 +113,16 @@ __device__ __forceinline__ void store_channels(const Int4Call& p, int64_t m, int
     }
 }
 
-// Channels n .. n + 3 of row m from their sums; NaN for a row that is none of x.
+// Channels n .. n + 3 of row m from their sums, which are in units of Op's
+// weights; NaN for a row that is none of x.
+template <class Op>
 __device__ __forceinline__ void store_sums(const Int4Call& p, int64_t m, int n, bool vec, v4f sum) {
     if (n >= p.N) return;
     const bool none = source_row(p, m) < 0;
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        y[i] = sum[i];
+        y[i] = sum[i] * Op::UNIT;
         if (p.bias) y[i] += bias_at(p, min(n + i, p.N - 1));
         if (none) y[i] = __builtin_nanf("");
     }
@@ -154,8 +156,11 @@ hipError_t by_int4_types(int x_dtype, int scale_dtype, int group, F f) {
     return scale_dtype == MI_LAYER_F32 ? steps(__bf16{}, float{}) : steps(__bf16{}, __bf16{});
 }
 
-enum class Int4Tile { Row, T32x64, T64x128, T128x128, T256x192 };
+// Rows x channels of a workgroup. T4x16 and T16x16 are those of int4_row.hip,
+// T256 that of int4_wide.hip.
+enum class Int4Tile { T4x16, T16x16, T16x32, T16x64, T16x128, T32x64, T32x128, T64x64, T64x128, T128x64, T128x128, T256, END };
 hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);
-hipError_t launch_int4_row(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hipStream_t s);
+hipError_t launch_int4_wide(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hipStream_t s);
+hipError_t launch_int4_row(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);
 
 }  // namespace miexp

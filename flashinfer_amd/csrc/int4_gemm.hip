@@ -35,32 +35,35 @@ bool int4_offsets_fit(const Int4Call& p) {
 
 Int4Tile pick_tile(const Int4Call& p) {
     const int64_t groups = p.offsets ? p.E : 1, rows = (p.rows + groups - 1) / groups;
-    if (rows <= 16) return Int4Tile::Row;
+    if (rows <= 4 && !p.offsets) return Int4Tile::T4x16;
+    if (rows <= 16) return p.offsets ? Int4Tile::T16x128 : Int4Tile::T16x16;
     if (rows <= 32) return Int4Tile::T32x64;
     if (rows <= 64) return Int4Tile::T64x128;
     auto tiles = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
     if (tiles(64, 128) <= 256) return Int4Tile::T64x128;
     if (tiles(128, 128) <= 256) return Int4Tile::T128x128;
-    return Int4Tile::T256x192;
+    return Int4Tile::T256;
 }
 
-// Whether a launch of this tile holds fewer than 2^32 threads.
+// Whether a launch of this tile holds fewer than 2^32 threads (of those of
+// int4_row.hip, 4096 workgroups go over any number).
 bool launch_fits(const Int4Call& p, Int4Tile tile) {
-    static const struct { int bm, bn, threads; } form[] = {{32, 64, 512}, {64, 128, 512}, {128, 128, 512}, {256, 192, 512}};
-    if (tile == Int4Tile::Row) return true;
-    const auto& f = form[(int)tile - 1];
+    static const struct { int bm, bn, threads; } form[] = {
+        {16, 32, 512}, {16, 64, 512}, {16, 128, 512}, {32, 64, 512}, {32, 128, 512}, {64, 64, 512},
+        {64, 128, 512}, {128, 64, 512}, {128, 128, 512}, {256, 128, 512}};
+    if (tile <= Int4Tile::T16x16) return true;
+    const auto& f = form[(int)tile - (int)Int4Tile::T16x32];
     return max_tiles(p.rows, f.bm, p.E) * ((p.N + f.bn - 1) / f.bn) * f.threads < (int64_t)1 << 32;
 }
 
-// MI_INT4_TILE = 0 .. 4 (an Int4Tile) takes that tile where a call can have it, for tests and timing.
+// MI_INT4_TILE = 0 .. 11 (an Int4Tile) takes that tile where a call can have it, for tests and timing.
 Int4Tile forced_tile(const Int4Call& p, Int4Tile tile) {
     const char* env = getenv("MI_INT4_TILE");
     if (env && *env) {
         const int v = atoi(env);
-        if (v>4) return (Int4Tile)v;
- if (v >= 0 && v <= (int)Int4Tile::T256x192) tile = (Int4Tile)v;
+        if (v >= 0 && v < (int)Int4Tile::END) tile = (Int4Tile)v;
     }
-    return launch_fits(p, tile) && int4_offsets_fit(p) ? tile : Int4Tile::Row;
+    return tile <= Int4Tile::T16x16 || (launch_fits(p, tile) && int4_offsets_fit(p)) ? tile : Int4Tile::T16x16;
 }
 
 hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
@@ -102,7 +105,8 @@ hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
     const uint64_t quad = a.out_dtype == MI_LAYER_F32 ? 16 : 8;
     const bool vec = (uint64_t)a.out % quad == 0 && a.out_stride % 4 == 0;
     const Int4Tile tile = forced_tile(p, pick_tile(p));
-    if (tile == Int4Tile::Row) return launch_int4_row(p, a.x_dtype, a.scale_dtype, vec, s);
+    if (tile <= Int4Tile::T16x16) return launch_int4_row(p, a.x_dtype, a.scale_dtype, tile, vec, s);
+    if (tile == Int4Tile::T256) return launch_int4_wide(p, a.x_dtype, a.scale_dtype, vec, s);
     return launch_int4_tile(p, a.x_dtype, a.scale_dtype, tile, vec, s);
 }
 

@@ -7,9 +7,7 @@
 // fragments from LDS (NT channel tiles share them), and adds each group's sums,
 // scaled, to its results. Per v_mfma_f32_16x16x32 of 16 cycles that takes
 // 256 / NT bytes of LDS a cycle and CU (of 128), and 52 / MT (bfloat16) and 16 /
-// GS cycles of a SIMD's other instructions (GS: its products per group). So
-// tiles of many rows go by 128 x 48 a wave, two waves to a SIMD: the most that
-// their 256 registers hold.
+// GS cycles of a SIMD's other instructions (GS: its products per group).
 //
 // LDS rows are 256 bytes, 16-byte chunk c of row r at position c ^ (r % 16);
 // weight tiles lie as in memory. Copies past K read the step's first chunk, and
@@ -141,7 +139,7 @@ void int4_tile_kernel(Int4Call p, int ntiles, int vec) {
             for (int j = 0; j < G; ++j) {
                 const s4 s = *reinterpret_cast<const s4*>(ss + (j * BN + n * 16 + 4 * g) * sizeof(ST));
 #pragma unroll
-                for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[v] * Op::UNIT;
+                for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[v];
             }
         }
 #pragma unroll
@@ -195,7 +193,7 @@ void int4_tile_kernel(Int4Call p, int ntiles, int vec) {
             const int row = (wm * MT + m) * 16 + r;
             if (row >= nrows) continue;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) store_sums(p, row0 + row, n0 + (wn * NT + n) * 16 + 4 * g, vec, acc[m][n]);
+            for (int n = 0; n < NT; ++n) store_sums<Op>(p, row0 + row, n0 + (wn * NT + n) * 16 + 4 * g, vec, acc[m][n]);
         }
     }
     zero_rest_any(p, vec);
@@ -215,16 +213,15 @@ hipError_t launch(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hip
 
 hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s) {
     switch (tile) {
+        case Int4Tile::T16x32: return launch<1, 1, 1, 2, 5, 4>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T16x64: return launch<1, 1, 1, 4, 4, 2>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T16x128: return launch<1, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T32x64: return launch<2, 1, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T32x128: return launch<2, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T64x64: return launch<4, 1, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T64x128: return launch<4, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
-        case Int4Tile::T128x128: return launch<4, 2, 2, 4, 3, 1>(p, x_dtype, scale_dtype, vec, s);
-        case (Int4Tile)5: return launch<1, 1, 1, 4, 4, 2>(p, x_dtype, scale_dtype, vec, s);
-        case (Int4Tile)6: return launch<1, 1, 1, 4, 4, 4>(p, x_dtype, scale_dtype, vec, s);
-        case (Int4Tile)7: return launch<1, 1, 1, 2, 5, 4>(p, x_dtype, scale_dtype, vec, s);
-        case (Int4Tile)8: return launch<1, 1, 1, 1, 3, 8>(p, x_dtype, scale_dtype, vec, s);
-        case (Int4Tile)9: return launch<1, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
-        case (Int4Tile)10: return launch<2, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
-        default: return launch<8, 3, 2, 4, 2, 1>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T128x64: return launch<8, 1, 1, 4, 2, 2>(p, x_dtype, scale_dtype, vec, s);
+        default: return launch<4, 2, 2, 4, 3, 1>(p, x_dtype, scale_dtype, vec, s);
     }
 }
 

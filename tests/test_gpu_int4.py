@@ -99,7 +99,7 @@ def test_matmul(shape, dtype):
     _check(fa.int4_matmul(x, w, bias=bias, out_dtype=torch.float32), x, full, bias)
 
 
-TILES = range(5)
+TILES = range(12)
 
 
 @pytest.mark.parametrize("tile", TILES)
