@@ -3,20 +3,20 @@
 // wave of each group to one, and take turns at making weights.
 //
 // A step is 128 values of K. A wave multiplies 128 rows by 48 channels (32 with
-// groups of less than 128): first it
-// makes 16 bits of its channels' weights in registers, then it goes over its
-// eight row tiles. That is two phases: A, the weights and row tiles 0 - 3, and B,
-// row tiles 4 - 7; a barrier ends each, and group 1 runs one behind group 0. So
-// while one wave of a SIMD makes weights (3 x 52 instructions for bfloat16) the
-// other one multiplies. Row tiles of 16 go to the groups in turn, so that a tile
-// with few rows keeps both busy.
+// groups of less than 128): first it makes 16 bits of its channels' weights in
+// registers, then it goes over its eight row tiles. That is two phases: A, the
+// weights and two row tiles, and B, the other six; a barrier ends each, and group
+// 1 runs one behind group 0. So while one wave of a SIMD makes weights (3 x 52
+// instructions for bfloat16, as long as three or four row tiles take) the other
+// one multiplies, and then both do. Row tiles of 16 go to the groups in turn, so
+// that a tile with few rows keeps both busy.
 //
-// Copies into LDS (two stages): a group's rows in halves, the ones that phase A
-// reads (low) and those of phase B (high), by its own waves; weights and scales
-// by group 0. Of step t, phase A issues high and the weights of t + 1 and phase B
-// low of t + 2, into what the phase before has read, so that rows have three
-// phases to arrive and weights two. All but what phase B issued has to be there
-// when it ends: that is what the next step reads.
+// Copies into LDS (two stages): a group's rows by its own waves, the ones that
+// phase A reads (low) and those of phase B (high); weights and scales by group 0.
+// Of step t, phase A issues high and the weights of t + 1 and phase B low of t +
+// 2, into what the phase before has read, so that rows have three phases to
+// arrive and weights two. All but what phase B issued has to be there when it
+// ends: that is what the next step reads.
 #include "int4_common.hpp"
 #include "lds_copy.hpp"
 
@@ -27,8 +27,9 @@ using mimoe::g2l4s;
 
 namespace wide4 {
 constexpr int MT = 8, WN = 4, BM = 256;
-constexpr int X_HALF = 64 * 256, X = 4 * X_HALF;  // bytes of rows: [group][low, high]
-constexpr int LOW = X_HALF / 1024 / WN;           // copies of a wave for half of its group's rows
+constexpr int ML = 2;                                        // row tiles of phase A
+constexpr int X_GROUP = BM / 2 * 256, X = 2 * X_GROUP;       // bytes of rows
+constexpr int XC = X_GROUP / 1024 / WN, LOW = XC * ML / MT;  // copies of a wave: of its group's rows, of those of A
 template <class ST, int GS>
 struct Shape {
     // With groups of 32 and 64 a wave has 32 channels: 48, their scales and the
@@ -63,35 +64,37 @@ __device__ __forceinline__ void wide_run(const Int4Call& p, uint8_t* smem, int e
     const int wn = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
     const int rest = p.K - (p.KT - 1) * 128;  // values of the last step: 8 .. 128
 
-    // Copy i of a half fills rows 4 (wn LOW + i) .. + 3 of its 64; lane l takes
-    // row l / 16, position l % 16. Group row j is row 32 (j / 16) + 16 GROUP + j %
-    // 16 of the tile; rows past the tile repeat its last one.
+    // A copy fills four rows of the group; lane l takes row l / 16, position l %
+    // 16. Group row j is row 32 (j / 16) + 16 GROUP + j % 16 of the tile; rows past
+    // the tile repeat its last one.
     const uint8_t* x_base = (const uint8_t*)p.x + (p.row_ids ? 0 : row0 * p.x_stride * 2);
-    uint32_t x_off[2][LOW];
+    uint32_t x_off[XC];
     const int chunk_of_lane = lane & 15;
+    auto group_row = [&](int i) __attribute__((always_inline)) {
+        return 4 * (i < LOW ? wn * LOW + i : WN * LOW + wn * (XC - LOW) + i - LOW);
+    };
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < LOW; ++i) {
-            const int j = h * 64 + 4 * (wn * LOW + i) + (lane >> 4);
-            const int m = min(32 * (j >> 4) + 16 * GROUP + (j & 15), nrows - 1);
-            const int64_t from = p.row_ids ? max(source_row(p, row0 + m), (int64_t)0) : m;
-            x_off[h][i] = (uint32_t)(from * p.x_stride) * 2 + (chunk_of_lane ^ (j & 15)) * 16;
-        }
+    for (int i = 0; i < XC; ++i) {
+        const int j = group_row(i) + (lane >> 4);
+        const int m = min(32 * (j >> 4) + 16 * GROUP + (j & 15), nrows - 1);
+        const int64_t from = p.row_ids ? max(source_row(p, row0 + m), (int64_t)0) : m;
+        x_off[i] = (uint32_t)(from * p.x_stride) * 2 + (chunk_of_lane ^ (j & 15)) * 16;
+    }
     // past K, in a last step that K ends in: the step's first chunk
     auto cut = [&](int i) __attribute__((always_inline)) {
-        const int chunk = chunk_of_lane ^ ((4 * (wn * LOW + i) + (lane >> 4)) & 15);
+        const int chunk = chunk_of_lane ^ ((group_row(i) + (lane >> 4)) & 15);
         return (uint32_t)(chunk * 8 >= rest ? chunk * 16 : 0);
     };
-    auto issue_rows = [&](int kb, int h) __attribute__((always_inline)) {
-        uint8_t* to = smem + (kb & 1) * Z::STAGE + (GROUP * 2 + h) * X_HALF + wn * LOW * 1024;
+    auto issue_rows = [&](int kb, auto high) __attribute__((always_inline)) {
+        constexpr int FROM = decltype(high)::value ? LOW : 0, TO = decltype(high)::value ? XC : LOW;
+        uint8_t* to = smem + (kb & 1) * Z::STAGE + GROUP * X_GROUP;
         const uint8_t* x = x_base + (int64_t)kb * 256;
         if (kb == p.KT - 1 && rest != 128) {
 #pragma unroll
-            for (int i = 0; i < LOW; ++i) g2l16s(x, x_off[h][i] - cut(i), to + i * 1024);
+            for (int i = FROM; i < TO; ++i) g2l16s(x, x_off[i] - cut(i), to + group_row(i) * 256);
         } else {
 #pragma unroll
-            for (int i = 0; i < LOW; ++i) g2l16s(x, x_off[h][i], to + i * 1024);
+            for (int i = FROM; i < TO; ++i) g2l16s(x, x_off[i], to + group_row(i) * 256);
         }
     };
     const uint8_t* w_base = p.w + e * p.w_expert;
@@ -122,81 +125,88 @@ __device__ __forceinline__ void wide_run(const Int4Call& p, uint8_t* smem, int e
         for (int n = 0; n < NT; ++n) acc[m][n] = (v4f){0.f, 0.f, 0.f, 0.f};
     frag w[NT][4];
     v4f scale[NT][G];
-    auto make_weights = [&](int kb) __attribute__((always_inline)) {
-        const uint8_t* sw = smem + (kb & 1) * Z::STAGE + X + wn * NT * 1024;
-        const uint8_t* ss = smem + (kb & 1) * Z::STAGE + X + W + wn * NT * 16 * sizeof(ST);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const v4u d = *reinterpret_cast<const v4u*>(sw + n * 1024 + lane * 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[n][i] = Op::weights(d[i]);
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                const s4 s = *reinterpret_cast<const s4*>(ss + (j * BN + n * 16 + 4 * g) * sizeof(ST));
-#pragma unroll
-                for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[v];
-            }
-        }
-    };
-    // Row tiles go one by one: a branch each, which also keeps the compiler from
-    // spreading the sums of several over more registers than there are.
-    auto fragments = [&](frag (&x)[4], const uint8_t* rows, auto last_c) __attribute__((always_inline)) {
+    // The compiler would sink each LDS read to its use and wait there for it: what
+    // a fence of the scheduler parts stays in this order.
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    frag x[2][4];
+    auto fragments = [&](int m, int kb, auto last_c) __attribute__((always_inline)) {
+        const uint8_t* rows = smem + (kb & 1) * Z::STAGE + GROUP * X_GROUP + (m * 16 + r) * 256;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = *reinterpret_cast<const frag*>(rows + r * 256 + ((4 * i + g) ^ r) * 16);
-            if (decltype(last_c)::value && 32 * i + 8 * g >= rest) x[i] = __builtin_bit_cast(frag, (v4u){0, 0, 0, 0});
+            x[m & 1][i] = *reinterpret_cast<const frag*>(rows + ((4 * i + g) ^ r) * 16);
+            if (decltype(last_c)::value && 32 * i + 8 * g >= rest) x[m & 1][i] = __builtin_bit_cast(frag, (v4u){0, 0, 0, 0});
         }
     };
-    auto multiply = [&](int kb, auto half, auto last_c) __attribute__((always_inline)) {
-        constexpr int H = decltype(half)::value;
-        const uint8_t* sx = smem + (kb & 1) * Z::STAGE + (GROUP * 2 + H) * X_HALF;
-        frag x[2][4];
-        fragments(x[0], sx, last_c);
+    auto make_weights = [&](int kb, auto last_c) __attribute__((always_inline)) {
+        const uint8_t* sw = smem + (kb & 1) * Z::STAGE + X + wn * NT * 1024;
+        const uint8_t* ss = smem + (kb & 1) * Z::STAGE + X + W + wn * NT * 16 * sizeof(ST);
+        v4u d[NT];
+        s4 s[NT][G];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            if (32 * (H * 4 + m) + 16 * GROUP >= nrows) break;
-            if (m < 3) fragments(x[(m + 1) & 1], sx + (m + 1) * 4096, last_c);
+        for (int n = 0; n < NT; ++n) {
+            d[n] = *reinterpret_cast<const v4u*>(sw + n * 1024 + lane * 16);
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                v4f t[NT];
+            for (int j = 0; j < G; ++j) s[n][j] = *reinterpret_cast<const s4*>(ss + (j * BN + n * 16 + 4 * g) * sizeof(ST));
+        }
+        fragments(0, kb, last_c);
+        fence();
 #pragma unroll
-                for (int n = 0; n < NT; ++n) t[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = j * GS; i < j * GS + GS; ++i)
+            for (int i = 0; i < 4; ++i) w[n][i] = Op::weights(d[n][i]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) t[n] = Op::mfma(w[n][i], x[m & 1][i], t[n]);
+            for (int j = 0; j < G; ++j)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[n][j][v];
+        }
+    };
+    // The row tiles of a phase; the fragments of each are read while the one before is multiplied.
+    auto multiply = [&](int kb, auto high, auto last_c) __attribute__((always_inline)) {
+        constexpr int FROM = decltype(high)::value ? ML : 0, TO = decltype(high)::value ? MT : ML;
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        acc[H * 4 + m][n][v] = fmaf(scale[n][j][v], t[n][v], acc[H * 4 + m][n][v]);
+        for (int m = FROM; m < TO; ++m) {
+            fence();
+            if (m + 1 < TO) fragments(m + 1, kb, last_c);
+            fence();
+            if (32 * m + 16 * GROUP < nrows) {
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        v4f t = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = j * GS; i < j * GS + GS; ++i) t = Op::mfma(w[n][i], x[m & 1][i], t);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[m][n][v] = fmaf(scale[n][j][v], t[v], acc[m][n][v]);
+                    }
             }
         }
     };
     auto step = [&](int t, auto last_c) __attribute__((always_inline)) {
         // A
         if (t + 1 < p.KT) {
-            issue_rows(t + 1, 1);
+            issue_rows(t + 1, IntC<1>{});
             if constexpr (GROUP == 0) issue_weights(t + 1);
         }
-        make_weights(t);
+        make_weights(t, last_c);
         multiply(t, IntC<0>{}, last_c);
-        __builtin_amdgcn_sched_barrier(0);
+        fence();
         phase_end();
         // B
-        if (t + 2 < p.KT) issue_rows(t + 2, 0);
+        if (t + 2 < p.KT) issue_rows(t + 2, IntC<0>{});
+        fragments(ML, t, last_c);
         multiply(t, IntC<1>{}, last_c);
-        __builtin_amdgcn_sched_barrier(0);
+        fence();
         if (t + 2 < p.KT)
             phase_end<LOW>();
         else
             phase_end<0>();
     };
     if constexpr (GROUP == 0) issue_weights(0);
-    issue_rows(0, 0);
-    issue_rows(0, 1);
+    issue_rows(0, IntC<0>{});
+    issue_rows(0, IntC<1>{});
     if (p.KT > 1) {
-        issue_rows(1, 0);
+        issue_rows(1, IntC<0>{});
         phase_end<LOW>();
     } else {
         phase_end<0>();
