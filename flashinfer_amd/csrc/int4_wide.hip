@@ -13,10 +13,10 @@
 //
 // Copies into LDS (two stages): a group's rows by its own waves, the ones that
 // phase A reads (low) and those of phase B (high); weights and scales by group 0.
-// Of step t, phase A issues high and the weights of t + 1 and phase B low of t +
-// 2, into what the phase before has read, so that rows have three phases to
-// arrive and weights two. All but what phase B issued has to be there when it
-// ends: that is what the next step reads.
+// Of step t, phase A issues the weights of t + 1, and phase B high of t + 1, one
+// beside each row tile, and low of t + 2: each into what has been read before. So
+// the copies have two phases at least to arrive; at the end of a phase the next
+// one's are waited for.
 #include "int4_common.hpp"
 #include "lds_copy.hpp"
 
@@ -37,6 +37,7 @@ struct Shape {
     static constexpr int NT = GS == 4 ? 3 : 2, BN = 16 * NT * WN;
     static constexpr int G = 4 / GS, W = BN * 64, S = (G * BN * (int)sizeof(ST) + 255) / 256 * 256;
     static constexpr int STAGE = X + W + S;
+    static constexpr int WC = NT + (S / 256 + WN - 1) / WN;  // copies of a wave: weights and scales
     static_assert(2 * STAGE <= 160 * 1024, "LDS budget");
 };
 }  // namespace wide4
@@ -85,17 +86,13 @@ __device__ __forceinline__ void wide_run(const Int4Call& p, uint8_t* smem, int e
         const int chunk = chunk_of_lane ^ ((group_row(i) + (lane >> 4)) & 15);
         return (uint32_t)(chunk * 8 >= rest ? chunk * 16 : 0);
     };
-    auto issue_rows = [&](int kb, auto high) __attribute__((always_inline)) {
-        constexpr int FROM = decltype(high)::value ? LOW : 0, TO = decltype(high)::value ? XC : LOW;
-        uint8_t* to = smem + (kb & 1) * Z::STAGE + GROUP * X_GROUP;
-        const uint8_t* x = x_base + (int64_t)kb * 256;
-        if (kb == p.KT - 1 && rest != 128) {
+    auto issue_row = [&](int kb, int i) __attribute__((always_inline)) {
+        const uint32_t off = x_off[i] - (kb == p.KT - 1 && rest != 128 ? cut(i) : 0);
+        g2l16s(x_base + (int64_t)kb * 256, off, smem + (kb & 1) * Z::STAGE + GROUP * X_GROUP + group_row(i) * 256);
+    };
+    auto issue_low = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = FROM; i < TO; ++i) g2l16s(x, x_off[i] - cut(i), to + group_row(i) * 256);
-        } else {
-#pragma unroll
-            for (int i = FROM; i < TO; ++i) g2l16s(x, x_off[i], to + group_row(i) * 256);
-        }
+        for (int i = 0; i < LOW; ++i) issue_row(kb, i);
     };
     const uint8_t* w_base = p.w + e * p.w_expert;
     const int last_tile = p.Np / 16 - 1;
@@ -110,7 +107,7 @@ __device__ __forceinline__ void wide_run(const Int4Call& p, uint8_t* smem, int e
             g2l16s(w_base + ((int64_t)min(n0 / 16 + t, last_tile) * p.KT + kb) * 1024, lane * 16, to + t * 1024);
         }
 #pragma unroll
-        for (int i = 0; i < (Z::S / 256 + WN - 1) / WN; ++i) {
+        for (int i = 0; i < Z::WC - NT; ++i) {
             const int c = (wn + i * WN) % (Z::S / 256), d = c * 64 + lane;
             const int row = min(G == 1 ? (kb * 128) >> p.group_shift : kb * G + d / D, last_group);
             g2l4s(s_base, (uint32_t)row * row_bytes + min(d % D * 4, row_bytes - n0 * (int)sizeof(ST) - 4),
@@ -160,13 +157,16 @@ __device__ __forceinline__ void wide_run(const Int4Call& p, uint8_t* smem, int e
                 for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[n][j][v];
         }
     };
-    // The row tiles of a phase; the fragments of each are read while the one before is multiplied.
-    auto multiply = [&](int kb, auto high, auto last_c) __attribute__((always_inline)) {
+    // The row tiles of a phase; the fragments of each are read while the one
+    // before is multiplied. MORE: a copy of the next step's high rows goes out
+    // beside each.
+    auto multiply = [&](int kb, auto high, auto more, auto last_c) __attribute__((always_inline)) {
         constexpr int FROM = decltype(high)::value ? ML : 0, TO = decltype(high)::value ? MT : ML;
 #pragma unroll
         for (int m = FROM; m < TO; ++m) {
             fence();
             if (m + 1 < TO) fragments(m + 1, kb, last_c);
+            if constexpr (decltype(more)::value) issue_row(kb + 1, LOW + m - FROM);
             fence();
             if (32 * m + 16 * GROUP < nrows) {
 #pragma unroll
@@ -181,39 +181,40 @@ __device__ __forceinline__ void wide_run(const Int4Call& p, uint8_t* smem, int e
                     }
             }
         }
+        fence();
     };
-    auto step = [&](int t, auto last_c) __attribute__((always_inline)) {
+    static_assert(XC - LOW == MT - ML, "a copy for each row tile of phase B");
+    // two more steps follow, one, or none
+    auto step = [&](int t, auto more2, auto more1) __attribute__((always_inline)) {
+        constexpr bool M2 = decltype(more2)::value, M1 = decltype(more1)::value;
+        typedef IntC<!M1> Last;
         // A
-        if (t + 1 < p.KT) {
-            issue_rows(t + 1, IntC<1>{});
-            if constexpr (GROUP == 0) issue_weights(t + 1);
-        }
-        make_weights(t, last_c);
-        multiply(t, IntC<0>{}, last_c);
-        fence();
-        phase_end();
+        make_weights(t, Last{});
+        if constexpr (M1 && GROUP == 0) issue_weights(t + 1);
+        multiply(t, IntC<0>{}, IntC<0>{}, Last{});
+        // high of this step is there: later are low of t + 1 and what this phase issued
+        phase_end<M1 ? LOW + (GROUP == 0 ? Z::WC : 0) : 0>();
         // B
-        if (t + 2 < p.KT) issue_rows(t + 2, IntC<0>{});
-        fragments(ML, t, last_c);
-        multiply(t, IntC<1>{}, last_c);
-        fence();
-        if (t + 2 < p.KT)
-            phase_end<LOW>();
-        else
-            phase_end<0>();
+        fragments(ML, t, Last{});
+        multiply(t, IntC<1>{}, more1, Last{});
+        if constexpr (M2) issue_low(t + 2);
+        // low and weights of t + 1 are there: later are its high and low of t + 2
+        phase_end<(M1 ? XC - LOW : 0) + (M2 ? LOW : 0)>();
     };
     if constexpr (GROUP == 0) issue_weights(0);
-    issue_rows(0, IntC<0>{});
-    issue_rows(0, IntC<1>{});
+    issue_low(0);
+#pragma unroll
+    for (int i = LOW; i < XC; ++i) issue_row(0, i);
     if (p.KT > 1) {
-        issue_rows(1, IntC<0>{});
-        phase_end<LOW>();
+        issue_low(1);
+        phase_end<XC>();
     } else {
-        phase_end<0>();
+        phase_end<XC - LOW>();
     }
     if constexpr (GROUP == 1) phase_end();
-    for (int t = 0; t < p.KT - 1; ++t) step(t, IntC<0>{});
-    step(p.KT - 1, IntC<1>{});
+    for (int t = 0; t < p.KT - 2; ++t) step(t, IntC<1>{}, IntC<1>{});
+    if (p.KT > 1) step(p.KT - 2, IntC<0>{}, IntC<1>{});
+    step(p.KT - 1, IntC<0>{}, IntC<0>{});
     if constexpr (GROUP == 0) phase_end();
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -230,14 +231,18 @@ __global__ __launch_bounds__(512, 2) void int4_wide_kernel(Int4Call p, int ntile
     constexpr int BN = Shape<ST, GS>::BN;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * Shape<ST, GS>::STAGE];
     Tiles tile;
-    const int mt = blockIdx.x / ntiles, n0 = (int)(blockIdx.x % ntiles) * BN;
-    if (!find_expert<BM>(p, mt, tile)) return zero_rest_any(p, vec);
-    const int64_t row0 = (int64_t)tile.row + (int64_t)(mt - tile.first) * BM;
-    const int nrows = (int)min((int64_t)BM, tile.end - row0);
-    if (threadIdx.x < 256)
-        wide_run<XT, ST, GS, 0>(p, smem, tile.e, row0, nrows, n0, vec);
-    else
-        wide_run<XT, ST, GS, 1>(p, smem, tile.e, row0, nrows, n0, vec);
+    const int mt = blockIdx.x / ntiles, nt = blockIdx.x % ntiles;
+    if (find_expert<BM>(p, mt, tile)) {
+        // an expert's rows in tiles of the same height: 270 rows cost less as 135 twice than as 256 and 14
+        const int rows = tile.end - tile.row, height = ((rows + tile.tiles - 1) / tile.tiles + 31) / 32 * 32;
+        const int from = (mt - tile.first) * height, nrows = min(height, rows - from);
+        if (nrows > 0) {
+            if (threadIdx.x < 256)
+                wide_run<XT, ST, GS, 0>(p, smem, tile.e, (int64_t)tile.row + from, nrows, nt * BN, vec);
+            else
+                wide_run<XT, ST, GS, 1>(p, smem, tile.e, (int64_t)tile.row + from, nrows, nt * BN, vec);
+        }
+    }
     zero_rest_any(p, vec);
 }
 
