@@ -128,42 +128,52 @@ void int4_tile_kernel(Int4Call p, int ntiles, int vec) {
         // this group's last step may be K's: products past K are zero; it may have none in this turn
         const int left = !decltype(last_c)::value ? 128 : t >= steps ? 0 : t * KS + ks == p.KT - 1 ? rest : 128;
         if (decltype(last_c)::value && left == 0) return;
-        frag w[NT][4];
+        // The compiler would sink each LDS read to its use and wait there for it: what
+        // a fence of the scheduler parts stays in this order.
+        auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+        frag w[NT][4], x[2][4];
         v4f scale[NT][G];
+        v4u d[NT];
+        s4 s[NT][G];
+        auto fragments = [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[m & 1][i] = *reinterpret_cast<const frag*>(sx + (m * 16 + r) * 256 + ((4 * i + g) ^ r) * 16);
+                if (decltype(last_c)::value && 32 * i + 8 * g >= left) x[m & 1][i] = __builtin_bit_cast(frag, (v4u){0, 0, 0, 0});
+            }
+        };
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const v4u d = *reinterpret_cast<const v4u*>(sw + n * 1024 + lane * 16);
+            d[n] = *reinterpret_cast<const v4u*>(sw + n * 1024 + lane * 16);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[n][i] = Op::weights(d[i]);
+            for (int j = 0; j < G; ++j) s[n][j] = *reinterpret_cast<const s4*>(ss + (j * BN + n * 16 + 4 * g) * sizeof(ST));
+        }
+        fragments(0);
+        fence();
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                const s4 s = *reinterpret_cast<const s4*>(ss + (j * BN + n * 16 + 4 * g) * sizeof(ST));
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[v];
-            }
+            for (int i = 0; i < 4; ++i) w[n][i] = Op::weights(d[n][i]);
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) scale[n][j][v] = (float)s[n][j][v];
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            frag x[4];
+            fence();
+            if (m + 1 < MT) fragments(m + 1);
+            fence();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = *reinterpret_cast<const frag*>(sx + (m * 16 + r) * 256 + ((4 * i + g) ^ r) * 16);
-                if (decltype(last_c)::value && 32 * i + 8 * g >= left) x[i] = __builtin_bit_cast(frag, (v4u){0, 0, 0, 0});
-            }
+            for (int j = 0; j < G; ++j)
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                v4f t[NT];
+                for (int n = 0; n < NT; ++n) {
+                    v4f t = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) t[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+                    for (int i = j * GS; i < j * GS + GS; ++i) t = Op::mfma(w[n][i], x[m & 1][i], t);
 #pragma unroll
-                for (int i = j * GS; i < j * GS + GS; ++i)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) t[n] = Op::mfma(w[n][i], x[i], t[n]);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[m][n][v] = fmaf(scale[n][j][v], t[n][v], acc[m][n][v]);
-            }
+                    for (int v = 0; v < 4; ++v) acc[m][n][v] = fmaf(scale[n][j][v], t[v], acc[m][n][v]);
+                }
         }
     };
     for (int t = 0; t < turns - 1; ++t) turn(t, IntC<0>{});
