@@ -29,8 +29,15 @@ struct Int4Call {
     int E;
     int bias_dtype, out_dtype;
     int zero_rest;
-    int w_large;      // the weights exceed the 256 MB of the last cache
+    int64_t from_rows, to_rows;  // a launch that finds another number of rows with experts does nothing
 };
+
+// Whether this launch is the one for the rows that experts have.
+__device__ __forceinline__ bool is_for_rows(const Int4Call& p) {
+    if (!p.offsets || (p.from_rows == 0 && p.to_rows > p.rows)) return true;
+    const int64_t n = clamped(p.offsets, p.E, p.rows) - clamped(p.offsets, 0, p.rows);
+    return n >= p.from_rows && n < p.to_rows;
+}
 
 // Element types of x: its fragments, its matrix instruction, and the eight
 // weights of a word.
@@ -158,7 +165,7 @@ hipError_t by_int4_types(int x_dtype, int scale_dtype, int group, F f) {
 
 // Rows x channels of a workgroup. T4x16 and T16x16 are those of int4_row.hip,
 // T256 that of int4_wide.hip.
-enum class Int4Tile { T4x16, T16x16, T16x32, T16x64, T16x128, T32x64, T32x128, T64x64, T64x128, T128x64, T128x128, T256, END };
+enum class Int4Tile { T4x16, T16x16, T16x32, T16x64, T16x128, T32x64, T32x128, T64x64, T64x128, T128x128, T256, END };
 hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);
 hipError_t launch_int4_wide(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hipStream_t s);
 hipError_t launch_int4_row(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);

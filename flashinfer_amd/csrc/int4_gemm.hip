@@ -33,37 +33,71 @@ bool int4_offsets_fit(const Int4Call& p) {
     return (p.row_ids ? p.a_rows : (int64_t)256) * p.x_stride * 2 < most && p.scale_expert * 4 < most;
 }
 
-Int4Tile pick_tile(const Int4Call& p) {
-    const int64_t groups = p.offsets ? p.E : 1, rows = (p.rows + groups - 1) / groups;
-    if (rows <= 4 && !p.offsets) return Int4Tile::T4x16;
-    if (rows <= 16) return p.offsets ? Int4Tile::T16x128 : Int4Tile::T16x16;
-    if (rows <= 32) return Int4Tile::T32x64;
-    if (rows <= 64) return Int4Tile::T64x128;
-    auto tiles = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+// Tiles of a dense product: the smallest that leave at most one workgroup for
+// each of the 256 CUs. What a call of few tiles waits for is the chain of one
+// workgroup's steps, and small tiles have more groups of waves that share K
+// (4096 x 7168: 1 row 7.7 us, 16 8.8, 32 11.5, with 16 x 64 tiles 17; 64 rows
+// 17.4, with 16 x 32 20.6; 100 20.2 / 23.7 with 16 x 64; 256 27.5 / 29.5 with 32 x
+// 64; 512 41 / 52 with 64 x 64; 1024 74 / 80 with 64 x 128). With short K two or
+// three workgroups of 16 x 128 to a CU do as well (130 x 7168 x 2048: 14 us, 17.4
+// with 64 x 128).
+Int4Tile pick_dense(const Int4Call& p) {
+    auto tiles = [&](int bm, int bn) { return ((p.rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+    if (p.rows <= 4 && tiles(4, 16) <= 512) return Int4Tile::T4x16;
+    if (tiles(16, 16) <= 256) return Int4Tile::T16x16;
+    if (tiles(16, 32) <= 256) return Int4Tile::T16x32;
+    if (tiles(16, 64) <= 256) return Int4Tile::T16x64;
+    if (tiles(32, 64) <= 256) return Int4Tile::T32x64;
+    if (p.K <= 2048 && tiles(16, 128) <= 512) return Int4Tile::T16x128;
+    if (tiles(64, 64) <= 256) return Int4Tile::T64x64;
     if (tiles(64, 128) <= 256) return Int4Tile::T64x128;
     if (tiles(128, 128) <= 256) return Int4Tile::T128x128;
-    return Int4Tile::T256;
+    // 256 x 192 tiles for half of the CUs take longer than several rounds of small
+    // ones (1500 rows 138 us, 119 with 64 x 128; 2048 135 / 159)
+    return tiles(256, 192) >= 160 ? Int4Tile::T256 : Int4Tile::T64x128;
+}
+
+// Rows of an expert on average up to which 32 x 128 tiles are taken, not those of
+// 256 rows (32 experts of 4096 x 7168: 33 rows 173 / 248 us, 66 rows 278 / 280).
+constexpr int64_t SMALL_ROWS = 48;
+
+// Tiles of experts' products. The host knows the rows of the result, of which a
+// shard's experts have a part (an eighth, if they are 32 of 256). Where that
+// decides, both kernels are launched and one finds that the rows are not its own.
+Int4Tile pick_grouped(const Int4Call& p, Int4Tile& large) {
+    const int64_t rows = (p.rows + p.E - 1) / p.E;
+    large = Int4Tile::END;
+    // 16 x 128 reads the weights at the rate of memory (64 tokens, 8 of 256 experts
+    // each, 32 of them here: 92 us for 425 MB)
+    if (rows <= 32) return Int4Tile::T16x128;
+    if (rows > 512) return Int4Tile::T256;
+    if (rows > SMALL_ROWS) large = Int4Tile::T256;
+    return Int4Tile::T32x128;
 }
 
 // Whether a launch of this tile holds fewer than 2^32 threads (of those of
 // int4_row.hip, 4096 workgroups go over any number).
 bool launch_fits(const Int4Call& p, Int4Tile tile) {
-    static const struct { int bm, bn, threads; } form[] = {
-        {16, 32, 512}, {16, 64, 512}, {16, 128, 512}, {32, 64, 512}, {32, 128, 512}, {64, 64, 512},
-        {64, 128, 512}, {128, 64, 512}, {128, 128, 512}, {256, 128, 512}};
-    if (tile <= Int4Tile::T16x16) return true;
+    static const struct { int bm, bn; } form[] = {{16, 32}, {16, 64}, {16, 128}, {32, 64}, {32, 128}, {64, 64},
+                                                  {64, 128}, {128, 128}, {256, 128}};
     const auto& f = form[(int)tile - (int)Int4Tile::T16x32];
-    return max_tiles(p.rows, f.bm, p.E) * ((p.N + f.bn - 1) / f.bn) * f.threads < (int64_t)1 << 32;
+    return max_tiles(p.rows, f.bm, p.E) * ((p.N + f.bn - 1) / f.bn) * 512 < (int64_t)1 << 32;
 }
 
-// MI_INT4_TILE = 0 .. 11 (an Int4Tile) takes that tile where a call can have it, for tests and timing.
-Int4Tile forced_tile(const Int4Call& p, Int4Tile tile) {
+hipError_t launch_one(const Int4Call& p, const mi_layer_int4_args& a, Int4Tile tile, hipStream_t s) {
+    const uint64_t quad = a.out_dtype == MI_LAYER_F32 ? 16 : 8;
+    const bool vec = (uint64_t)a.out % quad == 0 && a.out_stride % 4 == 0;
+    if (tile > Int4Tile::T16x16 && !(launch_fits(p, tile) && int4_offsets_fit(p))) tile = Int4Tile::T16x16;
+    if (tile <= Int4Tile::T16x16) return launch_int4_row(p, a.x_dtype, a.scale_dtype, tile, vec, s);
+    if (tile == Int4Tile::T256) return launch_int4_wide(p, a.x_dtype, a.scale_dtype, vec, s);
+    return launch_int4_tile(p, a.x_dtype, a.scale_dtype, tile, vec, s);
+}
+
+// MI_INT4_TILE = 0 .. 10 (an Int4Tile) takes that tile where a call can have it, for tests and timing.
+Int4Tile forced_tile() {
     const char* env = getenv("MI_INT4_TILE");
-    if (env && *env) {
-        const int v = atoi(env);
-        if (v >= 0 && v < (int)Int4Tile::END) tile = (Int4Tile)v;
-    }
-    return tile <= Int4Tile::T16x16 || (launch_fits(p, tile) && int4_offsets_fit(p)) ? tile : Int4Tile::T16x16;
+    const int v = env && *env ? atoi(env) : -1;
+    return v >= 0 && v < (int)Int4Tile::END ? (Int4Tile)v : Int4Tile::END;
 }
 
 hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
@@ -91,7 +125,8 @@ hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
     p.bias_dtype = a.bias_dtype;
     p.out_dtype = a.out_dtype;
     p.zero_rest = a.num_experts != 0 && a.zero_rest != 0;
-    p.w_large = (p.E ? p.E : 1) * p.w_expert > ((int64_t)256 << 20);
+    p.from_rows = 0;
+    p.to_rows = INT64_MAX;
     if (!int4_aligned(a)) {
         const int ld = (p.K + 7) / 8 * 8;
         hipLaunchKernelGGL(int4_copy_kernel, dim3((unsigned)(p.a_rows < MAX_BLOCKS ? p.a_rows : MAX_BLOCKS)), dim3(256),
@@ -102,12 +137,19 @@ hipError_t launch_int4_matmul(const mi_layer_int4_args& a, hipStream_t s) {
         p.x_stride = ld;
         p.K = ld;  // zeros past K
     }
-    const uint64_t quad = a.out_dtype == MI_LAYER_F32 ? 16 : 8;
-    const bool vec = (uint64_t)a.out % quad == 0 && a.out_stride % 4 == 0;
-    const Int4Tile tile = forced_tile(p, pick_tile(p));
-    if (tile <= Int4Tile::T16x16) return launch_int4_row(p, a.x_dtype, a.scale_dtype, tile, vec, s);
-    if (tile == Int4Tile::T256) return launch_int4_wide(p, a.x_dtype, a.scale_dtype, vec, s);
-    return launch_int4_tile(p, a.x_dtype, a.scale_dtype, tile, vec, s);
+    const Int4Tile forced = forced_tile();
+    if (forced != Int4Tile::END) return launch_one(p, a, forced, s);
+    if (!p.offsets) return launch_one(p, a, pick_dense(p), s);
+    Int4Tile large;
+    const Int4Tile tile = pick_grouped(p, large);
+    // a tile that does not fit is one kernel for all
+    if (large == Int4Tile::END || !int4_offsets_fit(p) || !launch_fits(p, tile)) return launch_one(p, a, tile, s);
+    p.to_rows = SMALL_ROWS * p.E;
+    const hipError_t e = launch_one(p, a, tile, s);
+    if (e != hipSuccess) return e;
+    p.from_rows = p.to_rows;
+    p.to_rows = INT64_MAX;
+    return launch_one(p, a, large, s);
 }
 
 }  // namespace miexp

@@ -48,6 +48,7 @@ void int4_tile_kernel(Int4Call p, int ntiles, int vec) {
     typedef typename Op::frag frag;
     constexpr int BM = Z::BM, BN = Z::BN, WAVES = Z::WAVES, G = Z::G, LD = Z::LD;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[Z::LDS];
+    if (!is_for_rows(p)) return;
     Tiles tile;
     const int mt = blockIdx.x / ntiles, n0 = (int)(blockIdx.x % ntiles) * BN;
     if (!find_expert<BM>(p, mt, tile)) return zero_rest_any(p, vec);
@@ -214,7 +215,9 @@ hipError_t launch(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hip
     return by_int4_types(x_dtype, scale_dtype, 1 << p.group_shift, [&](auto x, auto sc, auto gs) {
         constexpr int GS = decltype(gs)::value;
         constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
-        const int64_t nt = (p.N + BN - 1) / BN, tiles = max_tiles(p.rows, BM, p.E) * nt;
+        // a launch that is for at most so many rows needs no more workgroups
+        const int64_t nt = (p.N + BN - 1) / BN, rows = p.rows < p.to_rows ? p.rows : p.to_rows;
+        const int64_t tiles = max_tiles(rows, BM, p.E) * nt;
         hipLaunchKernelGGL((int4_tile_kernel<decltype(x), decltype(sc), GS, MT, NT, WM, WN, STAGES, KS>),
                            dim3((unsigned)tiles), dim3(64 * WM * WN * KS), 0, s, p, (int)nt, (int)vec);
         return hipGetLastError();
@@ -225,12 +228,11 @@ hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int
     switch (tile) {
         case Int4Tile::T16x32: return launch<1, 1, 1, 2, 5, 4>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T16x64: return launch<1, 1, 1, 4, 4, 2>(p, x_dtype, scale_dtype, vec, s);
-        case Int4Tile::T16x128: return launch<1, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T16x128: return launch<1, 2, 1, 4, 2, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T32x64: return launch<2, 1, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
-        case Int4Tile::T32x128: return launch<2, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
+        case Int4Tile::T32x128: return launch<2, 2, 1, 4, 2, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T64x64: return launch<4, 1, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
         case Int4Tile::T64x128: return launch<4, 2, 1, 4, 3, 2>(p, x_dtype, scale_dtype, vec, s);
-        case Int4Tile::T128x64: return launch<8, 1, 1, 4, 2, 2>(p, x_dtype, scale_dtype, vec, s);
         default: return launch<4, 2, 2, 4, 3, 1>(p, x_dtype, scale_dtype, vec, s);
     }
 }

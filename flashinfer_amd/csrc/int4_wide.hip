@@ -230,6 +230,7 @@ __global__ __launch_bounds__(512, 2) void int4_wide_kernel(Int4Call p, int ntile
     using namespace wide4;
     constexpr int BN = Shape<ST, GS>::BN;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * Shape<ST, GS>::STAGE];
+    if (!is_for_rows(p)) return;
     Tiles tile;
     const int mt = blockIdx.x / ntiles, nt = blockIdx.x % ntiles;
     if (find_expert<BM>(p, mt, tile)) {

@@ -99,7 +99,7 @@ def test_matmul(shape, dtype):
     _check(fa.int4_matmul(x, w, bias=bias, out_dtype=torch.float32), x, full, bias)
 
 
-TILES = range(12)
+TILES = range(11)
 
 
 @pytest.mark.parametrize("tile", TILES)
@@ -142,6 +142,20 @@ def test_every_tile_grouped(tile, monkeypatch):
             assert bool(y[40].isnan().all())
             y[40] = ref[40] = 0
         assert torch.equal(y.to(F64), ref) and lo == used + 5
+
+
+@pytest.mark.parametrize("used", [0, 1, 300, 767, 768, 1500, 3000])
+def test_experts_that_have_a_part_of_the_rows(used):
+    """The rows that the experts have, which the device alone knows, choose the tile: on both sides of the border."""
+    E, N, K, R = 16, 130, 264, 3000
+    cuts = torch.linspace(0, used, E + 1).round().to(torch.int32).cuda()
+    q, scale, x = _q((E, N, K), 1), _powers((E, N, 3), torch.bfloat16, 2), _whole((R, K), torch.bfloat16, 3)
+    torch.full((R, N), 9.0, device="cuda")  # a freed block that holds no zeros, for the result to get
+    y = fa.int4_grouped_matmul(x, fa.pack_int4(q, scale), cuts, out_dtype=torch.float32)
+    ref = torch.zeros(R, N, dtype=F64, device="cuda")
+    for e, (lo, hi) in enumerate(zip(cuts.tolist()[:-1], cuts.tolist()[1:])):
+        ref[lo:hi] = torch.matmul(x[lo:hi].to(F64), _dequant(q[e], scale[e], 128).t())
+    assert torch.equal(y.to(F64), ref)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
