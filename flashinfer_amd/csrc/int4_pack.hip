@@ -18,17 +18,26 @@ __device__ __forceinline__ Int4Word int4_word(int64_t i, int64_t nt, int64_t kt)
 // The even values in the low four nibbles, the odd ones in the high four.
 __device__ __forceinline__ int int4_place(int v) { return 4 * ((v >> 1) + 4 * (v & 1)); }
 
+// VEC: eight values are one load (32 x 4096 x 7168: 1720 us with a load each).
+template <bool VEC>
 __global__ __launch_bounds__(256) void pack_int4_kernel(const int8_t* __restrict__ q, int64_t expert_stride,
                                                         int64_t stride, int64_t words, int64_t N, int64_t K, int64_t nt,
                                                         int64_t kt, uint32_t* __restrict__ to) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
         const Int4Word a = int4_word(i, nt, kt);
         uint32_t d = 0;
-        if (a.n < N) {
-            const int8_t* from = q + a.e * expert_stride + a.n * stride;
+        if (a.n < N && a.k < K) {
+            const int8_t* from = q + a.e * expert_stride + a.n * stride + a.k;
+            int8_t x[8] = {};
+            if constexpr (VEC) {
+                *reinterpret_cast<uint64_t*>(x) = *reinterpret_cast<const uint64_t*>(from);
+            } else {
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
-                if (a.k + v < K) d |= (uint32_t)(max(-8, min(7, (int)from[a.k + v])) & 15) << int4_place(v);
+                for (int v = 0; v < 8; ++v)
+                    if (a.k + v < K) x[v] = from[v];
+            }
+#pragma unroll
+            for (int v = 0; v < 8; ++v) d |= (uint32_t)(max(-8, min(7, (int)x[v])) & 15) << int4_place(v);
         }
         to[i] = d;
     }
@@ -108,8 +117,10 @@ hipError_t launch_pack_int4(const int8_t* q, int64_t q_expert_stride, int64_t q_
                             int scale_dtype, int64_t E, int64_t N, int64_t K, int group, uint8_t* packed,
                             void* scale_out, hipStream_t s) {
     const int64_t nt = (N + 15) / 16, kt = (K + 127) / 128, words = E * nt * kt * 256;
-    hipLaunchKernelGGL(pack_int4_kernel, dim3(blocks_for(words, 256)), dim3(256), 0, s, q, q_expert_stride, q_stride,
-                       words, N, K, nt, kt, (uint32_t*)packed);
+    const bool vec = ((uint64_t)q | (uint64_t)q_expert_stride | (uint64_t)q_stride | (uint64_t)K) % 8 == 0;
+    auto pack = vec ? pack_int4_kernel<true> : pack_int4_kernel<false>;
+    hipLaunchKernelGGL(pack, dim3(blocks_for(words, 256)), dim3(256), 0, s, q, q_expert_stride, q_stride, words, N, K, nt,
+                       kt, (uint32_t*)packed);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     return by_out_type(scale_dtype, [&](auto t) {

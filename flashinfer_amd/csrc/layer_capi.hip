@@ -111,6 +111,9 @@ int mi_layer_balance(const mi_layer_balance_args* args, void* stream) {
     g_last_error[0] = 0;
     if (!args) return fail(MI_LAYER_ERR_INVALID, "%s: args is NULL", who);
     if (int rc = check_balance(who, *args, false)) return rc;
+    if (args->num_tokens * args->top_k > INT32_MAX)  // counts have 32 bits
+        return fail(MI_LAYER_ERR_INVALID, "%s: num_tokens %lld x top_k %d out of range", who,
+                    (long long)args->num_tokens, args->top_k);
     if (!args->loss || !args->counts || (args->num_tokens > 0 && !args->topk_ids))
         return fail(MI_LAYER_ERR_INVALID, "%s: NULL pointer argument", who);
     if (!aligned(args->loss, 4) || !aligned(args->counts, 4) || !aligned(args->topk_ids, 4))

@@ -13,6 +13,8 @@ with a forward-mode tangent are refused. There is no CPU path.
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from .experts import _Extension
@@ -78,7 +80,7 @@ def swiglu(x: torch.Tensor, dropout: float = 0.0, seed: int | torch.Tensor | Non
     if isinstance(seed, torch.Tensor):
         tensor = seed
     elif threshold:
-        number = int(seed)
+        number = operator.index(seed)
         if not -(1 << 63) <= number < 1 << 64:
             raise ValueError(f"seed must have 64 bits, got {number}")
         number -= (number >> 63) << 64 if number > 0 else 0

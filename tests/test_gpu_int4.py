@@ -296,6 +296,28 @@ def test_quantize(dtype):
     assert torch.equal(a.packed, b.packed) and torch.equal(a.scale, b.scale)
 
 
+def test_rows_past_32_bits():
+    """Gathered rows that start 4 GiB and more into x, and results past 2^31 elements."""
+    wide = torch.zeros(70000, 32768, dtype=torch.bfloat16, device="cuda")
+    x, ids = wide[:, :264], torch.tensor([0, 65535, 65536, 69999, 5], dtype=torch.int32, device="cuda")
+    x[ids.long()] = _whole((5, 264), torch.bfloat16, 1)
+    q, scale = _q((2, 40, 264), 2), _powers((2, 40, 3), torch.float32, 3)
+    w, offs = fa.pack_int4(q, scale), torch.tensor([0, 2, 5], dtype=torch.int32, device="cuda")
+    for tiles in (1, 60):  # few rows, and many
+        table = ids.repeat_interleave(tiles)
+        y = fa.int4_grouped_matmul(x, w, offs * tiles, row_ids=table, out_dtype=torch.float32)
+        for e, (lo, hi) in enumerate(((0, 2 * tiles), (2 * tiles, 5 * tiles))):
+            ref = torch.matmul(x[table[lo:hi].long()].to(F64), _dequant(q[e], scale[e], 128).t())
+            assert torch.equal(y[lo:hi].to(F64), ref)
+    del wide, x
+    M, N = 70000, 32768
+    x = _whole((M, 8), torch.float16, 1)
+    q = _q((N, 8), 2)
+    y = fa.int4_matmul(x, fa.pack_int4(q, torch.ones(N, 1, device="cuda"), 32))
+    for rows in (slice(0, 100), slice(65500, 65600), slice(M - 100, M)):
+        assert torch.equal(y[rows].to(F64), torch.matmul(x[rows].to(F64), q.to(F64).t()))
+
+
 def test_graph_replays_and_streams():
     """Captured with a copy of unaligned rows: every replay equals the eager result, two graphs keep apart."""
     R, N, K = 50, 96, 330

@@ -130,6 +130,15 @@ def test_balance_sequences_and_masks(score):
     _check_balance(logits, ids, [0, 10, 33], none, score)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_balance_more_slots_than_lanes(score):
+    """More slots for a token than lanes hold it, and than there are experts."""
+    for T, E, k in ((50, 8, 33), (5000, 30, 64), (3, 2, 9)):
+        ids = torch.randint(-2, E + 2, (T, k), generator=_gen(T), device="cuda", dtype=torch.int32)
+        for dtype in (torch.float32, torch.bfloat16):
+            _check_balance(_randn((T, E), dtype, T), ids, [0, T], None, score, given_cuts=False)
+
+
 def test_balance_far_scores():
     """Rows of -inf, rows whose sigmoids leave fp32, a masked expert, large scores."""
     E = 20
@@ -338,7 +347,8 @@ def test_refusals():
         (TypeError, lambda: fa.swiglu(x.double())), (ValueError, lambda: fa.swiglu(x.cpu())),
         (ValueError, lambda: fa.swiglu(x, dropout=1.0, seed=1)), (ValueError, lambda: fa.swiglu(x, dropout=-0.1, seed=1)),
         (ValueError, lambda: fa.swiglu(x, dropout=float("nan"), seed=1)), (ValueError, lambda: fa.swiglu(x, dropout=0.1)),
-        (ValueError, lambda: fa.swiglu(x, dropout=0.1, seed=2**64)), (TypeError, lambda: fa.swiglu(x, 0.1, n)),
+        (ValueError, lambda: fa.swiglu(x, dropout=0.1, seed=2**64)), (TypeError, lambda: fa.swiglu(x, dropout=0.1, seed=1.5)),
+        (TypeError, lambda: fa.swiglu(x, 0.1, n)),
         (ValueError, lambda: fa.swiglu(x, 0.1, torch.zeros(2, dtype=torch.int64, device="cuda"))),
         (ValueError, lambda: fa.swiglu(x, 0.1, torch.zeros(1, dtype=torch.int64))),
         (TypeError, lambda: fa.swiglu(x, num_rows=n.long())), (ValueError, lambda: fa.swiglu(x, num_rows=n.expand(2))),

@@ -81,7 +81,7 @@ def test_balance_refuses():
             (dict(seq_offsets=None), "num_seqs"), (dict(logits_stride=-1), "stride")]
     refused("mi_layer_balance", Balance, good, both + [
         (dict(topk_ids=None), "NULL"), (dict(loss=None), "NULL"), (dict(counts=None), "NULL"),
-        (dict(topk_ids=P + 2), "misaligned"), (dict(top_k=0), "top_k"), (dict(top_k=65), "top_k"),
+        (dict(topk_ids=P + 2), "misaligned"), (dict(top_k=0), "top_k"), (dict(top_k=65), "top_k"), (dict(num_tokens=1 << 30), "num_tokens"),
         (dict(workspace=P + 16), "misaligned")], None)
     refused("mi_layer_balance", Balance, good, [(dict(workspace=None), "workspace"),
                                                 (dict(workspace_bytes=need - 1), "workspace")], None, code=2)
