@@ -14,6 +14,12 @@
 // sequence, in columns of experts where there are many; a third the columns and
 // the sequences, where there are more than one. All sums are in a fixed order;
 // the only atomics count whole numbers.
+//
+// 65536 x 256 in fp32 with sigmoids: pieces 19 us (3.6 TB/s), their sums 9 and 3,
+// gradient 24 (5.7 TB/s: a read and a write of 67 MB). A wave keeps up to four
+// tokens on their way; exponentials and quotients are the hardware's with one
+// correction, sums over lanes go by DPP. 64 x 256: 4.4, 4 and 3.5 us, all latency;
+// there a training step takes what autograd takes on the host, 53 us.
 #include "layer_common.hpp"
 
 namespace miexp {

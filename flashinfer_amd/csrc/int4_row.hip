@@ -8,6 +8,10 @@
 // tiles ahead of their use, and waits for nothing but its own copies; the waves'
 // sums meet at the end. Addresses are 64 bits for each lane, so this kernel also
 // takes what the 32-bit offsets of int4_tile.hip do not reach, with 16 rows.
+//
+// 1 x 4096 x 7168 7.1 to 7.7 us, 6.1 on the GPU: 2.7 of a launch that does nothing,
+// 1.6 of making weights and what the loads of 14.7 MB take beside it. (Loads into
+// registers instead: 8.9, and 13.2 with 16 rows, here 8.8.)
 #include "int4_common.hpp"
 #include "lds_copy.hpp"
 

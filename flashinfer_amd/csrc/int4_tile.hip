@@ -8,6 +8,12 @@
 // scaled, to its results. Per v_mfma_f32_16x16x32 of 16 cycles that takes
 // 256 / NT bytes of LDS a cycle and CU (of 128), and 52 / MT (bfloat16) and 16 /
 // GS cycles of a SIMD's other instructions (GS: its products per group).
+// So the smallest tiles are bound by making weights (a step of a wave with 16
+// rows x 16 channels takes about 530 cycles, whatever the memory's latency: each
+// SIMD's two to four waves take turns), those between by copies of rows too (about
+// 20 bytes a cycle and CU), and experts' weights that are read once by memory: 64
+// tokens, 8 of 256 experts each, 32 of them here, 4096 x 7168: 91 us with 16 x 128
+// (425 MB of weights, 4.7 TB/s), 97 with three stages, 125 with 32 x 64.
 //
 // LDS rows are 256 bytes, 16-byte chunk c of row r at position c ^ (r % 16);
 // weight tiles lie as in memory. Copies past K read the step's first chunk, and
