@@ -120,19 +120,24 @@ __device__ __forceinline__ void store_channels(const Int4Call& p, int64_t m, int
     }
 }
 
-// Channels n .. n + 3 of row m from their sums, which are in units of Op's
-// weights; NaN for a row that is none of x.
+// Results of channels n .. n + 3 of row m from their sums, which are in units of
+// Op's weights; NaN for a row that is none of x.
 template <class Op>
-__device__ __forceinline__ void store_sums(const Int4Call& p, int64_t m, int n, bool vec, v4f sum) {
-    if (n >= p.N) return;
+__device__ __forceinline__ void finish_sums(const Int4Call& p, int64_t m, int n, v4f sum, float (&y)[4]) {
     const bool none = source_row(p, m) < 0;
-    float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         y[i] = sum[i] * Op::UNIT;
         if (p.bias) y[i] += bias_at(p, min(n + i, p.N - 1));
         if (none) y[i] = __builtin_nanf("");
     }
+}
+
+template <class Op>
+__device__ __forceinline__ void store_sums(const Int4Call& p, int64_t m, int n, bool vec, v4f sum) {
+    if (n >= p.N) return;
+    float y[4];
+    finish_sums<Op>(p, m, n, sum, y);
     if (p.out_dtype == MI_LAYER_F32)
         store_channels<float>(p, m, n, vec, y);
     else if (p.out_dtype == MI_LAYER_F16)
@@ -167,7 +172,7 @@ hipError_t by_int4_types(int x_dtype, int scale_dtype, int group, F f) {
 // T256 that of int4_wide.hip.
 enum class Int4Tile { T4x16, T16x16, T16x32, T16x64, T16x128, T32x64, T32x128, T64x64, T64x128, T128x128, T256, END };
 hipError_t launch_int4_tile(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);
-hipError_t launch_int4_wide(const Int4Call& p, int x_dtype, int scale_dtype, bool vec, hipStream_t s);
+hipError_t launch_int4_wide(const Int4Call& p, int x_dtype, int scale_dtype, hipStream_t s);
 hipError_t launch_int4_row(const Int4Call& p, int x_dtype, int scale_dtype, Int4Tile tile, bool vec, hipStream_t s);
 
 }  // namespace miexp

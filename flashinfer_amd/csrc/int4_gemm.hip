@@ -89,7 +89,7 @@ hipError_t launch_one(const Int4Call& p, const mi_layer_int4_args& a, Int4Tile t
     const bool vec = (uint64_t)a.out % quad == 0 && a.out_stride % 4 == 0;
     if (tile > Int4Tile::T16x16 && !(launch_fits(p, tile) && int4_offsets_fit(p))) tile = Int4Tile::T16x16;
     if (tile <= Int4Tile::T16x16) return launch_int4_row(p, a.x_dtype, a.scale_dtype, tile, vec, s);
-    if (tile == Int4Tile::T256) return launch_int4_wide(p, a.x_dtype, a.scale_dtype, vec, s);
+    if (tile == Int4Tile::T256) return launch_int4_wide(p, a.x_dtype, a.scale_dtype, s);
     return launch_int4_tile(p, a.x_dtype, a.scale_dtype, tile, vec, s);
 }
 

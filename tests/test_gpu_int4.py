@@ -115,6 +115,11 @@ def test_every_tile(tile, monkeypatch):
                 scale = _powers((N, -(-K // group)), scale_type, n + 2)
                 y = fa.int4_matmul(x, fa.pack_int4(q, scale, group), out_dtype=torch.float32)
                 assert torch.equal(y.to(F64), torch.matmul(x.to(F64), _dequant(q, scale, group).t())), (M, N, K, group)
+                # results of 16 bits are these, rounded; in rows of a multiple of 16 bytes, too
+                assert torch.equal(fa.int4_matmul(x, fa.pack_int4(q, scale, group)), y.to(dtype))
+                buf = torch.full((M, -(-N // 8) * 8 + 8), 9.0, dtype=dtype, device="cuda")
+                fa.int4_matmul(x, fa.pack_int4(q, scale, group), out=buf[:, :N])
+                assert torch.equal(buf[:, :N], y.to(dtype)) and bool((buf[:, N:] == 9).all())
 
 
 @pytest.mark.parametrize("tile", TILES)
@@ -142,6 +147,12 @@ def test_every_tile_grouped(tile, monkeypatch):
             assert bool(y[40].isnan().all())
             y[40] = ref[40] = 0
         assert torch.equal(y.to(F64), ref) and lo == used + 5
+        half = torch.full((R, N), 9.0, dtype=torch.float16, device="cuda")
+        fa.int4_grouped_matmul(rows, w, offs, row_ids=table, out=half)
+        if table is not None:
+            assert bool(half[40].isnan().all())
+            half[40] = 0
+        assert torch.equal(half[5:lo], ref[5:lo].to(torch.float16)) and bool((half[:5] == 9).all() & (half[lo:] == 9).all())
 
 
 @pytest.mark.parametrize("used", [0, 1, 300, 767, 768, 1500, 3000])
