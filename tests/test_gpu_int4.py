@@ -116,7 +116,10 @@ def test_every_tile(tile, monkeypatch):
                 y = fa.int4_matmul(x, fa.pack_int4(q, scale, group), out_dtype=torch.float32)
                 assert torch.equal(y.to(F64), torch.matmul(x.to(F64), _dequant(q, scale, group).t())), (M, N, K, group)
                 # results of 16 bits are these, rounded; in rows of a multiple of 16 bytes, too
-                assert torch.equal(fa.int4_matmul(x, fa.pack_int4(q, scale, group)), y.to(dtype))
+                w = fa.pack_int4(q, scale, group)
+                assert torch.equal(fa.int4_matmul(x, w), y.to(dtype))
+                bias = torch.arange(N, device="cuda", dtype=torch.float32) - 7
+                assert torch.equal(fa.int4_matmul(x, w, bias=bias, out_dtype=torch.bfloat16), (y + bias).bfloat16())
                 buf = torch.full((M, -(-N // 8) * 8 + 8), 9.0, dtype=dtype, device="cuda")
                 fa.int4_matmul(x, fa.pack_int4(q, scale, group), out=buf[:, :N])
                 assert torch.equal(buf[:, :N], y.to(dtype)) and bool((buf[:, N:] == 9).all())
@@ -153,6 +156,17 @@ def test_every_tile_grouped(tile, monkeypatch):
             assert bool(half[40].isnan().all())
             half[40] = 0
         assert torch.equal(half[5:lo], ref[5:lo].to(torch.float16)) and bool((half[:5] == 9).all() & (half[lo:] == 9).all())
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("shape", [(8200, 4100, 136), (5000, 5555, 264), (33000, 777, 128)], ids=str)
+def test_many_large_tiles(shape, group):
+    """Several rounds of the largest tiles."""
+    M, N, K = shape
+    q, x = _q((N, K), 1), _whole((M, K), torch.bfloat16, 2)
+    scale = _powers((N, -(-K // group)), torch.bfloat16, 3)
+    y = fa.int4_matmul(x, fa.pack_int4(q, scale, group), out_dtype=torch.float32)
+    assert torch.equal(y.to(F64), torch.matmul(x.to(F64), _dequant(q, scale, group).t()))
 
 
 @pytest.mark.parametrize("used", [0, 1, 300, 767, 768, 1500, 3000])
