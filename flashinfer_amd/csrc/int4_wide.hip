@@ -18,13 +18,13 @@
 // the copies have two phases at least to arrive; at the end of a phase the next
 // one's are waited for.
 //
-// 8192 x 4096 x 7168 446 to 462 us (1.05 to 1.08 PFLOP/s; the library's product of
+// 8192 x 4096 x 7168 435 to 445 us (1.08 to 1.11 PFLOP/s; the library's product of
 // bfloat16 weights 372), in groups of 64 478 to 500, of 32 590 to 603; 8192 rows of
-// 32 experts of 7168 x 2048 310 to 328. Without the copies the first takes 392, without
-// making weights 408, without storing results 421: no one part holds it; 704 tiles
-// are two and three quarters rounds of the CUs. Before: all eight row tiles behind
-// the weights in one phase 500, four in each phase 486, the copies of a step all at
-// its start 472.
+// 32 experts of 7168 x 2048 300 to 325. Where the first took 446, 392 without the
+// copies, 408 without making weights, 421 without storing results: no one part
+// holds it; 704 tiles are two and three quarters rounds of the CUs. Before: all
+// eight row tiles behind the weights in one phase 500, four in each phase 486, the
+// copies of a step all at its start 472, stores of four channels 446.
 #include "int4_common.hpp"
 #include "lds_copy.hpp"
 
