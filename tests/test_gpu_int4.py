@@ -294,6 +294,19 @@ def test_values_that_are_not_finite(M):
     assert torch.equal(y[0].to(F64), torch.matmul(x[:1, :129].to(F64), q[:, :129].to(F64).t())[0])
 
 
+@pytest.mark.parametrize("M", [3, 16, 70, 600])
+def test_small_values(M):
+    """float16 below its normal range (its steps of 2^-24), bfloat16 far below 1: multiplied as they are."""
+    N, K = 200, 256
+    q, one = _q((N, K), 1), torch.ones(N, 2, device="cuda")
+    w = fa.pack_int4(q, one)
+    for dtype, unit in ((torch.float16, 2.0 ** -24), (torch.bfloat16, 2.0 ** -100)):
+        x = (_whole((M, K), torch.float32, 2) * unit).to(dtype)
+        assert x.any()
+        y = fa.int4_matmul(x, w, out_dtype=torch.float32)
+        assert torch.equal(y.to(F64), torch.matmul(x.to(F64), q.to(F64).t()))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
 def test_quantize(dtype):
     for shape, group in (((40, 200), 32), ((3, 17, 1000), 128), ((5, 64), 4096), ((1, 1), 32)):
