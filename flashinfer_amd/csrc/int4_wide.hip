@@ -48,6 +48,13 @@ struct Shape {
     static constexpr int WC = NT + (S / 256 + WN - 1) / WN;  // copies of a wave: weights and scales
     static_assert(2 * STAGE <= 160 * 1024, "LDS budget");
 };
+// Rows of each of `tiles` tiles that share `rows` evenly, in 32s: at most BM,
+// as there are ceil(rows / BM). Up to 2^31 - 1 rows, so nothing is added to them
+// before the division.
+constexpr int tile_height(int rows, int tiles) { return ((rows - 1) / tiles + 32) / 32 * 32; }
+static_assert(tile_height(1, 1) == 32 && tile_height(256, 1) == 256 && tile_height(257, 2) == 160 &&
+                  tile_height(270, 2) == 160 && tile_height(2147483392, 8388607) == BM,
+              "all rows in tiles of at most BM");
 }  // namespace wide4
 
 // End of a phase: this wave's LDS reads are done and at most N of its copies
@@ -294,7 +301,7 @@ __global__ __launch_bounds__(512, 2) void int4_wide_kernel(Int4Call p, int ntile
     const int mt = blockIdx.x / ntiles, nt = blockIdx.x % ntiles;
     if (find_expert<BM>(p, mt, tile)) {
         // an expert's rows in tiles of the same height: 270 rows cost less as 135 twice than as 256 and 14
-        const int rows = tile.end - tile.row, height = ((rows + tile.tiles - 1) / tile.tiles + 31) / 32 * 32;
+        const int rows = tile.end - tile.row, height = wide4::tile_height(rows, tile.tiles);
         const int from = (mt - tile.first) * height, nrows = min(height, rows - from);
         if (nrows > 0) {
             if (threadIdx.x < 256)

@@ -1,0 +1,31 @@
+"""Products with 4-bit weights of as many rows as a call can have: 32 bits hold
+their number, and not much more. Every row is one row of x at distance 0, so
+that results alone take memory."""
+import pytest
+import torch
+
+import flashinfer_amd as fa
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def _equal_everywhere(y, value):
+    return all(bool((part == value).all()) for part in y.view(-1).split(1 << 28))
+
+
+@pytest.mark.parametrize("rows", [2139127681, 2147483391])
+def test_dense_rows_up_to_32_bits(rows):
+    """From the first number of rows that passes 31 bits with their 8355968 tiles of 256 added."""
+    K = 32
+    x = torch.arange(-5, K - 5, device="cuda").to(torch.bfloat16)[None]
+    q = torch.full((1, K), 3, dtype=torch.int8, device="cuda")
+    w = fa.pack_int4(q, torch.full((1, 1), 0.5, device="cuda"), 32)
+    out = torch.full((rows, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
+    fa.int4_matmul(x.expand(rows, K), w, out=out)
+    assert _equal_everywhere(out, 1.5 * sum(range(-5, K - 5)))  # 504, exact in bfloat16
