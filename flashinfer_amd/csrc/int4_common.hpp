@@ -53,21 +53,23 @@ __device__ __forceinline__ bool is_for_rows(const Int4Call& p) {
 template <class XT> struct Operand;
 
 // v_cvt_off_f32_i4 makes q / 16 of the low 4 bits in two's complement, and the
-// upper half of that is it in bfloat16: 13 instructions for eight values.
+// upper half of that is it in bfloat16: 13 instructions for eight values, as it
+// can take its bits from any byte. As a builtin, not in assembly: behind a matrix
+// instruction that still reads its addend from the registers that a vector
+// instruction writes there have to be wait states, which the compiler counts for
+// its own instructions alone.
 template <> struct Operand<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
     static constexpr float UNIT = 16.f;  // weights are made as sixteenths, and sums are multiplied at their end
     __device__ __forceinline__ static frag weights(uint32_t d) {
-        const uint32_t h = d >> 4;
+        uint32_t h = d >> 4;
+        asm("" : "+v"(h));  // bytes of this word, not bit fields of d: they cost an instruction less
         float e[8];  // nibbles 0 .. 7
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_0" : "=v"(e[0]) : "v"(d));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_0" : "=v"(e[1]) : "v"(h));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_1" : "=v"(e[2]) : "v"(d));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_1" : "=v"(e[3]) : "v"(h));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_2" : "=v"(e[4]) : "v"(d));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_2" : "=v"(e[5]) : "v"(h));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_3" : "=v"(e[6]) : "v"(d));
-        asm("v_cvt_off_f32_i4_sdwa %0, %1 src0_sel:BYTE_3" : "=v"(e[7]) : "v"(h));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            e[2 * i] = __builtin_amdgcn_cvt_off_f32_i4((int)(d >> 8 * i & 0xffu));
+            e[2 * i + 1] = __builtin_amdgcn_cvt_off_f32_i4((int)(h >> 8 * i & 0xffu));
+        }
         v4u r;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
