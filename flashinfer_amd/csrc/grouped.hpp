@@ -19,6 +19,13 @@ struct Tiles {
     int row, end;   // its rows
 };
 
+// ceil(rows / BM) for up to 2^31 - 1 rows: BM - 1 more may have no place in 32 bits.
+template <int BM>
+constexpr int tiles_for(int rows) { return rows / BM + (rows % BM != 0); }
+static_assert(tiles_for<16>(0) == 0 && tiles_for<16>(1) == 1 && tiles_for<16>(16) == 1 && tiles_for<16>(17) == 2 &&
+                  tiles_for<4>(2147483647) == 536870912 && tiles_for<256>(2147483647) == 8388608,
+              "a tile for every row");
+
 // Row tiles of lane's expert e0 + lane (none past the last), and their inclusive sum.
 template <int BM, class Call>
 __device__ __forceinline__ int scan_tiles(const Call& p, int e0, int& lo, int& hi, int& inc) {
@@ -28,7 +35,7 @@ __device__ __forceinline__ int scan_tiles(const Call& p, int e0, int& lo, int& h
         lo = (int)clamped(p.offsets, x, p.rows);
         hi = max(lo, (int)clamped(p.offsets, x + 1, p.rows));
     }
-    const int tiles = (hi - lo + BM - 1) / BM;
+    const int tiles = tiles_for<BM>(hi - lo);
     inc = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {

@@ -19,7 +19,7 @@ def _equal_everywhere(y, value):
     return all(bool((part == value).all()) for part in y.view(-1).split(1 << 28))
 
 
-@pytest.mark.parametrize("rows", [2139127681, 2147483391])
+@pytest.mark.parametrize("rows", [2139127681, 2147483391, 2147483647])
 def test_dense_rows_up_to_32_bits(rows):
     """From the first number of rows that passes 31 bits with their 8355968 tiles of 256 added."""
     K = 32
@@ -28,4 +28,16 @@ def test_dense_rows_up_to_32_bits(rows):
     w = fa.pack_int4(q, torch.full((1, 1), 0.5, device="cuda"), 32)
     out = torch.full((rows, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
     fa.int4_matmul(x.expand(rows, K), w, out=out)
-    assert _equal_everywhere(out, 1.5 * sum(range(-5, K - 5)))  # 504, exact in bfloat16
+    assert _equal_everywhere(out, 504.0)  # 1.5 times the sum of -5 .. 26, exact in bfloat16
+
+
+@pytest.mark.parametrize("rows", [2147483633, 2147483647])
+def test_an_expert_with_rows_up_to_32_bits(rows):
+    """From the first number of rows that passes 31 bits with 15 added."""
+    K = 32
+    x = torch.arange(-5, K - 5, device="cuda").to(torch.bfloat16)[None]
+    q = torch.full((1, 1, K), 3, dtype=torch.int8, device="cuda")
+    w = fa.pack_int4(q, torch.full((1, 1, 1), 0.5, device="cuda"), 32)
+    out = torch.full((rows, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
+    fa.int4_grouped_matmul(x.expand(rows, K), w, torch.tensor([0, rows], dtype=torch.int32, device="cuda"), out=out)
+    assert _equal_everywhere(out, 504.0)
