@@ -40,24 +40,33 @@ __device__ __forceinline__ void g2l4(const void* gsrc, void* lds_base) {
 // The same two copies with a wave-uniform 64-bit base in SGPRs and a 32-bit
 // per-lane byte offset (the saddr form: address = sbase + voff): one VGPR per
 // copy instead of a 64-bit address per lane.
+//
+// The base may come from a vector instruction (a readfirstlane, the reload of a
+// spilled SGPR), and a vector memory access reads such an SGPR rightly only five
+// wait states later, which the compiler does not put in front of assembly. A
+// scalar instruction is made to wait for it, so the copies go by a scalar move
+// of the base, which is M0's wait state, too.
 __device__ __forceinline__ void g2l16s(const void* sbase, uint32_t voff, void* lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :
+    uint64_t base;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(base)
                  : "v"(voff), "s"(sbase), "s"(lds_addr(lds_base))
                  : "memory", "m0");
 }
 
 // g2l16s for data that nothing reads again: it leaves nothing in the caches.
 __device__ __forceinline__ void g2l16s_once(const void* sbase, uint32_t voff, void* lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
-                 :
+    uint64_t base;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0 nt"
+                 : "=&s"(base)
                  : "v"(voff), "s"(sbase), "s"(lds_addr(lds_base))
                  : "memory", "m0");
 }
 
 __device__ __forceinline__ void g2l4s(const void* sbase, uint32_t voff, void* lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
-                 :
+    uint64_t base;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dword %1, %0"
+                 : "=&s"(base)
                  : "v"(voff), "s"(sbase), "s"(lds_addr(lds_base))
                  : "memory", "m0");
 }
