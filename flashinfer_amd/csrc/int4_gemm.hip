@@ -37,10 +37,15 @@ bool int4_offsets_fit(const Int4Call& p) {
 // each of the 256 CUs. What a call of few tiles waits for is the chain of one
 // workgroup's steps, and small tiles have more groups of waves that share K
 // (4096 x 7168: 1 row 7.7 us, 16 8.8, 32 11.5, with 16 x 64 tiles 17; 64 rows
-// 17.4, with 16 x 32 20.6; 100 20.2 / 23.7 with 16 x 64; 256 27.5 / 29.5 with 32 x
-// 64; 512 41 / 52 with 64 x 64; 1024 74 / 80 with 64 x 128). With short K two or
-// three workgroups of 16 x 128 to a CU do as well (130 x 7168 x 2048: 14 us, 17.4
-// with 64 x 128).
+// 17.4, with 16 x 32 20.6; 100 20.2 / 23.7 with 16 x 64; 256 26 / 27.6 with 32 x
+// 64; 512 41 / 52 with 64 x 64; 1024 74 / 80 with 64 x 128).
+// Where 64 x 64 tiles do not fit, two workgroups of a smaller one to a CU do better
+// than one of 64 x 128, whatever K is (in groups of 128; 2048 / 7168 values of K; 160
+// rows x 6144: 11.4 / 28.2 us with 480 tiles of 32 x 64, 13.6 / 36.5 with 480 of 16 x
+// 128, 15.2 / 38.6 with 64 x 128; 144 x 7168: 16.0 / 41.6 with 560 of 32 x 64, 13.7 /
+// 36.2 with 504 of 16 x 128, 15.2 / 38.7; 210 x 4700: 16.4 / 41.6 with 518 of 32 x 64,
+// 20.0 / 55.7 with 518 of 16 x 128, 15.6 / 38.8); where they fit, one of those does
+// (256 x 4096: 10.7 / 26.0, 13.5 / 35.5 with 512 of 16 x 128).
 Int4Tile pick_dense(const Int4Call& p) {
     auto tiles = [&](int bm, int bn) { return ((p.rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
     if (p.rows <= 4 && tiles(4, 16) <= 512) return Int4Tile::T4x16;
@@ -48,13 +53,17 @@ Int4Tile pick_dense(const Int4Call& p) {
     if (tiles(16, 32) <= 256) return Int4Tile::T16x32;
     if (tiles(16, 64) <= 256) return Int4Tile::T16x64;
     if (tiles(32, 64) <= 256) return Int4Tile::T32x64;
-    if (p.K <= 2048 && tiles(16, 128) <= 512) return Int4Tile::T16x128;
     if (tiles(64, 64) <= 256) return Int4Tile::T64x64;
+    if (tiles(32, 64) <= 512) return Int4Tile::T32x64;
+    if (tiles(16, 128) <= 512) return Int4Tile::T16x128;
     if (tiles(64, 128) <= 256) return Int4Tile::T64x128;
     if (tiles(128, 128) <= 256) return Int4Tile::T128x128;
-    // 256 x 192 tiles for half of the CUs take longer than several rounds of small
-    // ones (1500 rows 138 us, 119 with 64 x 128; 2048 135 / 159)
-    return tiles(256, 192) >= 160 ? Int4Tile::T256 : Int4Tile::T64x128;
+    // A round of 256 x 192 tiles takes as long as three and a half of 64 x 128 ones
+    // (4096 x 7168: 1500 rows, three rounds, 115 us / 134 with 256 x 192, 1750, four, 152 /
+    // 135; 2048 x 1024: 2600 rows, three, 29.8 / 30.9, 3500, four, 38.9 / 30.5), one of 256
+    // x 128 in smaller groups less than three (groups of 64, 1100 rows of 4096 x 7168, 114 /
+    // 98, 1500 117 / 111, 2200 of 2048 x 1024 30 / 24).
+    return p.group_shift >= 7 && tiles(64, 128) <= 3 * 256 ? Int4Tile::T64x128 : Int4Tile::T256;
 }
 
 // Rows of an expert on average up to which 32 x 128 tiles are taken, not those of

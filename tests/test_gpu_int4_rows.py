@@ -1,6 +1,7 @@
-"""Products with 4-bit weights of as many rows as a call can have: 32 bits hold
-their number, and not much more. Every row is one row of x at distance 0, so
-that results alone take memory."""
+"""Products with 4-bit weights on both sides of the borders between tiles, and of
+as many rows as a call can have: 32 bits hold their number, and not much more.
+There every row is one row of x at distance 0, so that results alone take
+memory."""
 import pytest
 import torch
 
@@ -41,3 +42,24 @@ def test_an_expert_with_rows_up_to_32_bits(rows):
     out = torch.full((rows, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
     fa.int4_grouped_matmul(x.expand(rows, K), w, torch.tensor([0, rows], dtype=torch.int32, device="cuda"), out=out)
     assert _equal_everywhere(out, 504.0)
+
+
+# rows, channels: the last of a tile and the first of the next
+BORDERS = [(64, 2048), (65, 2048), (128, 4096), (129, 4096), (256, 4096), (257, 4096), (160, 6144), (161, 6144),
+           (144, 7168), (145, 7168), (204, 4700), (512, 2048), (513, 2048), (1024, 2048), (1025, 2048),
+           (1536, 4096), (1537, 4096), (2048, 2048)]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("shape", BORDERS, ids=str)
+def test_borders_between_tiles(shape, group):
+    """Whole numbers: every element counts once, whatever the order of the sums."""
+    (M, N), K = shape, 264
+    dtype = torch.bfloat16 if M % 2 else torch.float16
+    g = torch.Generator(device="cuda").manual_seed(M)
+    q = torch.empty((N, K), dtype=torch.int8, device="cuda").random_(-8, 8, generator=g)
+    x = torch.empty((M, K), device="cuda").random_(-4, 5, generator=g).to(dtype)
+    scale = torch.empty((N, -(-K // group)), device="cuda").random_(0, 2, generator=g).exp2()
+    y = fa.int4_matmul(x, fa.pack_int4(q, scale, group), out_dtype=torch.float32)
+    w = q.double() * scale.double()[:, torch.arange(K, device="cuda") // group]
+    assert torch.equal(y.double(), torch.matmul(x.double(), w.t()))
