@@ -67,8 +67,11 @@ Int4Tile pick_dense(const Int4Call& p) {
 }
 
 // Rows of an expert on average up to which 32 x 128 tiles are taken, not those of
-// 256 rows (32 experts of 4096 x 7168: 33 rows 173 / 248 us, 66 rows 278 / 280).
-constexpr int64_t SMALL_ROWS = 48;
+// 256 rows (32 experts with a router's spread; 4096 x 7168 in groups of 128: 56
+// rows 194 us / 274, 80 271 / 277, 88 295 / 280, 112 349 / 304; in groups of 32 56
+// rows 226 / 326, 80 300 / 340, 112 399 / 386; 7168 x 2048 56 rows 116 / 151, 80 151 /
+// 160, 96 179 / 164).
+constexpr int SMALL_ROWS = 80;
 
 // Tiles of experts' products. The host knows the rows of the result, of which a
 // shard's experts have a part (an eighth, if they are 32 of 256). Where that
@@ -77,7 +80,7 @@ Int4Tile pick_grouped(const Int4Call& p, Int4Tile& large) {
     const int64_t rows = (p.rows + p.E - 1) / p.E;
     large = Int4Tile::END;
     // 16 x 128 reads the weights at the rate of memory (64 tokens, 8 of 256 experts
-    // each, 32 of them here: 92 us for 425 MB)
+    // each, 32 of them here: 87 us for 425 MB)
     if (rows <= 32) return Int4Tile::T16x128;
     if (rows > 512) return Int4Tile::T256;
     if (rows > SMALL_ROWS) large = Int4Tile::T256;

@@ -63,3 +63,21 @@ def test_borders_between_tiles(shape, group):
     y = fa.int4_matmul(x, fa.pack_int4(q, scale, group), out_dtype=torch.float32)
     w = q.double() * scale.double()[:, torch.arange(K, device="cuda") // group]
     assert torch.equal(y.double(), torch.matmul(x.double(), w.t()))
+
+
+@pytest.mark.parametrize("used", [0, 800, 1279, 1280, 1281, 2999])
+def test_experts_on_both_sides_of_the_large_tiles(used):
+    """80 rows of an expert on average: the rows that the experts have, which the device alone knows, choose."""
+    E, N, K, R = 16, 130, 264, 3000
+    cuts = torch.linspace(0, used, E + 1).round().to(torch.int32).cuda()
+    g = torch.Generator(device="cuda").manual_seed(used)
+    q = torch.empty((E, N, K), dtype=torch.int8, device="cuda").random_(-8, 8, generator=g)
+    x = torch.empty((R, K), device="cuda").random_(-4, 5, generator=g).to(torch.bfloat16)
+    scale = torch.empty((E, N, 3), device="cuda").random_(0, 2, generator=g).exp2()
+    torch.full((R, N), 9.0, device="cuda")  # a freed block that holds no zeros, for the result to get
+    y = fa.int4_grouped_matmul(x, fa.pack_int4(q, scale), cuts, out_dtype=torch.float32)
+    w = q.double() * scale.double()[..., torch.arange(K, device="cuda") // 128]
+    ref = torch.zeros(R, N, dtype=torch.float64, device="cuda")
+    for e, (lo, hi) in enumerate(zip(cuts.tolist()[:-1], cuts.tolist()[1:])):
+        ref[lo:hi] = torch.matmul(x[lo:hi].double(), w[e].t())
+    assert torch.equal(y.double(), ref)
