@@ -82,7 +82,9 @@ template <> struct Operand<__bf16> {
 };
 
 // The bits of q + 8 as the last ones of 1024 (or, 4 bits up, as sixteenths of
-// it), and 1032 off again: 9 instructions for eight values.
+// it), and 1032 off again: 9 instructions for eight values. The way of Kim,
+// Henry, Fahim, Awadalla: Who says elephants can't run: bringing large scale MoE
+// models into cloud scale production (2022); the numbers follow from the format.
 template <> struct Operand<_Float16> {
     typedef _Float16 frag __attribute__((ext_vector_type(8)));
     static constexpr float UNIT = 1.f;

@@ -18,8 +18,8 @@
 // the copies have two phases at least to arrive; at the end of a phase the next
 // one's are waited for.
 //
-// 8192 x 4096 x 7168 435 to 445 us (1.08 to 1.11 PFLOP/s; the library's product of
-// bfloat16 weights 372), in groups of 64 478 to 500, of 32 590 to 603; 8192 rows of
+// 8192 x 4096 x 7168 430 to 450 us (1.07 to 1.12 PFLOP/s; the library's product of
+// bfloat16 weights 372), in groups of 64 470 to 500, of 32 590 to 603; 8192 rows of
 // 32 experts of 7168 x 2048 300 to 325. Where the first took 446, 392 without the
 // copies, 408 without making weights, 421 without storing results: no one part
 // holds it; 704 tiles are two and three quarters rounds of the CUs. Before: all

@@ -13,6 +13,9 @@
 // Memory bounds it: 65536 x 2048 in bf16 with dropout 157 us (5.1 TB/s), its
 // gradient 218 (6.1 TB/s); 18006 x 1536 in fp16 36 and 48. Ten rounds of two
 // products, sixteen selects and the gate for eight columns stay below that.
+// Rows that are not whole vectors of 16 bytes, or not aligned to them, go one
+// element at a time: 65536 x 2047 in bf16 415 and 730 us, 18006 x 1535 82 and 145
+// (1.8 to 2 TB/s).
 #include "layer_common.hpp"
 
 namespace miexp {
